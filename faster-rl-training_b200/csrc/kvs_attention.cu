@@ -503,6 +503,8 @@ KVS_API size_t kvs_abi_struct_size(int which) {
     case 2: return sizeof(kvs_decode_args);
     case 3: return sizeof(kvs_replay_args);
     case 4: return sizeof(kvs_segments);
+    case 5: return sizeof(kvs_linear_args);
+    case 6: return sizeof(kvs_linear_grads);
   }
   return 0;
 }

@@ -168,6 +168,47 @@ class KvsSegments(C.Structure):
     ]
 
 
+class KvsLinearArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("weight_up", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("residual", C.c_void_p),
+        ("pre", C.c_void_p),
+        ("out", C.c_void_p),
+        ("ld_x", C.c_int64),
+        ("ld_w", C.c_int64),
+        ("ld_w_up", C.c_int64),
+        ("ld_res", C.c_int64),
+        ("ld_pre", C.c_int64),
+        ("ld_out", C.c_int64),
+        ("rows", C.c_int32),
+        ("n", C.c_int32),
+        ("k", C.c_int32),
+        ("dtype", C.c_int32),
+        ("activation", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class KvsLinearGrads(C.Structure):
+    _fields_ = [
+        ("gy", C.c_void_p),
+        ("dx", C.c_void_p),
+        ("dw", C.c_void_p),
+        ("dw_up", C.c_void_p),
+        ("db", C.c_void_p),
+        ("scratch", C.c_void_p),
+        ("scratch_bytes", C.c_size_t),
+        ("ld_gy", C.c_int64),
+        ("ld_dx", C.c_int64),
+        ("ld_dw", C.c_int64),
+    ]
+
+
+ACTIVATION_CODES = {None: 0, "relu": 1, "silu": 2, "gelu": 3}  # kvs_activation
+
 SIGNATURES = {
     "kvs_abi_struct_size": (_Z, [C.c_int]),
     "kvs_abi_version": (C.c_int, []),
@@ -213,9 +254,16 @@ SIGNATURES = {
     "kvs_lm_head_logprobs_supported": (C.c_int, [_I]),
     "kvs_lm_head_logprobs": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _I, _I, _I, _P, C.c_double, _P, _P, _P, _Z,
                                        _P]),
+    "kvs_linear": (C.c_int, [_P, _P]),
+    "kvs_linear_backward_scratch_bytes": (_Z, [_P, _P]),
+    "kvs_linear_backward": (C.c_int, [_P, _P, _P]),
+    "kvs_distill": (C.c_int, [_P, C.c_int64, _I, _I, _P, _P, _I, C.c_double, _I, _P, _P, _P]),
+    "kvs_distill_backward": (C.c_int, [_P, C.c_int64, _I, _I, _P, _P, _I, _P, _P, C.c_double, _I, _P, C.c_int64, _I,
+                                       _P]),
 }
 
-STRUCTS = {0: KvsCache, 1: KvsBatch, 2: KvsDecodeArgs, 3: KvsReplayArgs, 4: KvsSegments}
+STRUCTS = {0: KvsCache, 1: KvsBatch, 2: KvsDecodeArgs, 3: KvsReplayArgs, 4: KvsSegments, 5: KvsLinearArgs,
+           6: KvsLinearGrads}
 
 _lock = threading.Lock()
 _lib: C.CDLL | None = None

@@ -453,3 +453,272 @@ def silu_mul_backward(gu: torch.Tensor, grad: torch.Tensor) -> torch.Tensor:
                                        N.stream_ptr(gu.device))
     N.check(rc, "kvs_silu_mul_backward")
     return dgu.view(gu.shape)
+
+
+# ---------------------------------------------------------------------- layer products
+class _on:
+    """Makes the device of ``t`` current for a launch (nothing to do when it already is)."""
+
+    __slots__ = ("want", "prev")
+
+    def __init__(self, t: torch.Tensor) -> None:
+        self.want = t.device.index
+
+    def __enter__(self) -> None:
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.want:
+            torch.cuda.set_device(self.want)
+
+    def __exit__(self, *exc) -> None:
+        if self.prev != self.want:
+            torch.cuda.set_device(self.prev)
+
+
+def _matrix(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """``t`` as ``[rows, cols]`` rows that the products' copies can read where they lie (dense
+    columns, a row pitch that is a multiple of 8, a 16-byte aligned base), else a copy."""
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
+    if t.stride(1) != 1 or t.data_ptr() % 16 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < cols)):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _same(name: str, t: torch.Tensor, like: torch.Tensor, shape) -> None:
+    if t.dtype != like.dtype or t.device != like.device or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be a {like.dtype} tensor of shape {tuple(shape)} on {like.device} "
+                         f"(got {t.dtype} {tuple(t.shape)} on {t.device})")
+
+
+def _dense_rows(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """``t`` as ``[rows, cols]`` with dense columns and rows that do not overlap, else a copy."""
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
+    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _out_rows(name: str, t: torch.Tensor, cols: int) -> torch.Tensor:
+    """An output buffer as ``[rows, cols]`` without copying; raises where that cannot be done."""
+    t2 = t.view(-1, cols) if t.dim() != 2 else t  # view raises on rows that do not line up
+    if (cols > 1 and t2.stride(1) != 1) or (t2.shape[0] > 1 and t2.stride(0) < cols):
+        raise ValueError(f"{name} needs dense, non-overlapping rows")
+    return t2
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _product_args(x, weight, weight_up, activation):
+    """Checked operands of a product: the C arguments, the matrices they point into."""
+    if not (x.is_cuda and weight.is_cuda):
+        _check_cuda(x, weight)
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
+    n, k = weight.shape
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"layer products take bfloat16 or float16 (got {x.dtype})")
+    if k == 0 or k % 8 or n == 0:
+        raise ValueError(f"layer products need an inner size that is a multiple of 8 and outputs (got {n} x {k})")
+    _same("weight", weight, x, (n, k))
+    code = N.ACTIVATION_CODES.get(activation)
+    if code is None:
+        raise ValueError(f"unknown activation {activation!r}: one of {list(N.ACTIVATION_CODES)}")
+    x2, w2 = _matrix(x, k), _matrix(weight, k)
+    a = N.KvsLinearArgs(x=x2.data_ptr(), weight=w2.data_ptr(), ld_x=_ld(x2), ld_w=_ld(w2), rows=x2.shape[0], n=n,
+                        k=k, dtype=N.DTYPE_CODE[x.dtype], activation=code)
+    keep = [x2, w2]
+    if weight_up is not None:
+        _same("w_up", weight_up, x, (n, k))
+        u2 = _matrix(weight_up, k)
+        a.weight_up, a.ld_w_up = u2.data_ptr(), _ld(u2)
+        keep.append(u2)
+    return a, keep
+
+
+def pre_buffer(x: torch.Tensor, width: int) -> torch.Tensor:
+    """Buffer for the pre-activations of a product of ``x``: ``[..., width]`` of its type."""
+    return torch.empty(*x.shape[:-1], width, dtype=x.dtype, device=x.device)
+
+
+def _product(x, weight, weight_up, activation, bias, residual, pre, out):
+    a, keep = _product_args(x, weight, weight_up, activation)
+    n, lead = a.n, x.shape[:-1]
+    if out is None:
+        out = torch.empty(*lead, n, dtype=x.dtype, device=x.device)
+    else:
+        _same("out", out, x, (*lead, n))
+    o2 = _out_rows("out", out, n)
+    a.out, a.ld_out = o2.data_ptr(), _ld(o2)
+    if bias is not None:
+        _same("bias", bias, x, (n,))
+        b = bias.contiguous()
+        a.bias = b.data_ptr()
+        keep.append(b)
+    if residual is not None:
+        _same("residual", residual, x, (*lead, n))
+        r2 = _dense_rows(residual, n)
+        a.residual, a.ld_res = r2.data_ptr(), _ld(r2)
+        keep.append(r2)
+    if pre is not None:
+        width = n if weight_up is None else 2 * n
+        _same("pre", pre, x, (*lead, width))
+        p2 = _out_rows("pre", pre, width)
+        a.pre, a.ld_pre = p2.data_ptr(), _ld(p2)
+    with _on(x):
+        N.check(N.lib().kvs_linear(C.byref(a), N.stream_ptr(x.device)), "kvs_linear")
+    return out
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+           residual: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+           pre: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual`` in one launch for bf16/fp16 CUDA tensors: float32
+    accumulation and epilogue, one rounding.  x ``[..., k]`` (k a multiple of 8), weight ``[n, k]``,
+    bias ``[n]``, residual ``[..., n]``; ``activation`` None, "relu", "silu" or "gelu" (erf form).
+    ``pre`` (:func:`pre_buffer` of width n) receives ``x @ weight.T + bias`` for
+    :func:`linear_backward`; ``out`` may be the residual itself."""
+    return _product(x, weight, None, activation, bias, residual, pre, out)
+
+
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: Optional[str] = "silu",
+                 pre: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act(x @ w_gate.T) * (x @ w_up.T)`` (model.py:78-86 before the down projection) in one
+    launch, both projections, activation and product: the gate|up tensor is never stored, nor are
+    the weights concatenated.  ``pre`` (:func:`pre_buffer` of width 2n) receives gate|up, which
+    :func:`gated_linear_backward` needs."""
+    return _product(x, w_gate, w_up, activation, None, None, pre, out)
+
+
+def _product_backward(gy, x, weight, weight_up, pre, activation, bias_grad):
+    a, keep = _product_args(x, weight, weight_up, activation)
+    n, k, lead = a.n, a.k, x.shape[:-1]
+    _same("the upstream gradient", gy, x, (*lead, n))
+    g2 = _dense_rows(gy, n)
+    if weight_up is not None or activation is not None:
+        if pre is None:
+            raise ValueError("the backward of an activation needs the forward's pre buffer")
+        width = n if weight_up is None else 2 * n
+        _same("pre", pre, x, (*lead, width))
+        p2 = _dense_rows(pre, width)
+        a.pre, a.ld_pre = p2.data_ptr(), _ld(p2)
+        keep.append(p2)
+    dx = torch.empty(*lead, k, dtype=x.dtype, device=x.device)
+    dw = torch.empty(n, k, dtype=x.dtype, device=x.device)
+    du = torch.empty_like(dw) if weight_up is not None else None
+    db = torch.empty(n, dtype=x.dtype, device=x.device) if bias_grad else None
+    g = N.KvsLinearGrads(gy=g2.data_ptr(), dx=dx.data_ptr(), dw=dw.data_ptr(), ld_gy=_ld(g2), ld_dx=k, ld_dw=k)
+    if du is not None:
+        g.dw_up = du.data_ptr()
+    if db is not None:
+        g.db = db.data_ptr()
+    lib = N.lib()
+    nbytes = int(lib.kvs_linear_backward_scratch_bytes(C.byref(a), C.byref(g)))
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    if scratch is not None:
+        g.scratch, g.scratch_bytes = scratch.data_ptr(), nbytes
+    with _on(x):
+        N.check(lib.kvs_linear_backward(C.byref(a), C.byref(g), N.stream_ptr(x.device)), "kvs_linear_backward")
+    return dx, dw, du, db
+
+
+def linear_backward(gy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre: Optional[torch.Tensor] = None,
+                    activation: Optional[str] = None, bias_grad: bool = False):
+    """``(dx, dw, db)``: gradients of :func:`linear` for the upstream ``gy`` (``db`` None unless
+    ``bias_grad``; the residual's gradient is ``gy`` itself).  An activation needs the forward's
+    ``pre``.  ``gy act'(pre)`` is rounded to the operands' type for the products; sums run in
+    float32 in a fixed order and are rounded once."""
+    dx, dw, _, db = _product_backward(gy, x, weight, None, pre, activation, bias_grad)
+    return dx, dw, db
+
+
+def gated_linear_backward(gh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
+                          pre: torch.Tensor, activation: Optional[str] = "silu"):
+    """``(dx, dw_gate, dw_up)``: gradients of :func:`gated_linear` for the upstream ``gh`` with the
+    forward's gate|up ``pre``."""
+    dx, dg, du, _ = _product_backward(gh, x, w_gate, w_up, pre, activation, False)
+    return dx, dg, du
+
+
+# ---------------------------------------------------------------------- distillation
+def _distill_args(logits, ids, teacher):
+    _check_cuda(logits, ids, teacher)
+    if logits.dtype not in N.DTYPE_CODE:
+        raise ValueError(f"unsupported logits dtype {logits.dtype}")
+    if logits.dim() != 2 or logits.shape[1] == 0 or logits.stride(1) != 1:
+        raise ValueError("logits must be a 2-D tensor with contiguous rows")
+    if ids.dim() != 2 or ids.shape[0] != logits.shape[0] or ids.shape[1] == 0 or tuple(teacher.shape) != tuple(ids.shape):
+        raise ValueError(f"ids and teacher must be [{logits.shape[0]}, top] "
+                         f"(got {tuple(ids.shape)} and {tuple(teacher.shape)})")
+    if ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
+        raise ValueError(f"ids must be integers (got {ids.dtype})")
+    if ids.device != logits.device or teacher.device != logits.device:
+        raise ValueError("logits, ids and teacher must be on one device")
+    acc = torch.float64 if logits.dtype == torch.float64 else torch.float32
+    if logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]:  # an expanded row
+        logits = logits.contiguous()
+    return logits, ids.to(torch.long).contiguous(), teacher.to(acc).contiguous(), acc
+
+
+def distill(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, temperature: float = 1.0):
+    """``(loss, lse)`` of the student's rows against a teacher's top logits: ``ids`` ``[rows, top]``
+    and ``teacher`` ``[rows, top]`` (raw logits or log-probs) name the teacher's best entries of
+    each row; with ``p = softmax(teacher / T)`` over a row's kept slots,
+
+        loss = sum_j p_j (log p_j - log_softmax(logits / T)[ids_j]),   lse = logsumexp(logits / T)
+
+    A slot with a negative id, or a teacher value of -inf or NaN, is empty; a row without kept
+    slots has loss 0.  One pass over each row; float32 results (float64 for float64 logits)."""
+    logits, i, t, acc = _distill_args(logits, ids, teacher)
+    n, vocab = logits.shape
+    loss = torch.empty(n, dtype=acc, device=logits.device)
+    lse = torch.empty(n, dtype=acc, device=logits.device)
+    with _on(logits):
+        rc = N.lib().kvs_distill(logits.data_ptr(), _ld(logits), n, vocab, i.data_ptr(), t.data_ptr(), i.shape[1],
+                                 float(temperature), N.DTYPE_CODE[logits.dtype], loss.data_ptr(), lse.data_ptr(),
+                                 N.stream_ptr(logits.device))
+    N.check(rc, "kvs_distill")
+    return loss, lse
+
+
+def distill_backward(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, lse: torch.Tensor,
+                     grad: torch.Tensor, temperature: float = 1.0, out_dtype: Optional[torch.dtype] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of :func:`distill`'s loss with respect to the logits for upstream ``grad`` ``[rows]``
+    and the forward's ``lse``, in ``out_dtype`` (the logits' type; bf16 / fp16 from float32 logits).
+    ``out`` may be ``logits`` itself.  Rows without kept slots get zeros."""
+    given = logits
+    logits, i, t, acc = _distill_args(logits, ids, teacher)
+    n, vocab = logits.shape
+    for name, v in (("lse", lse), ("grad", grad)):
+        if tuple(v.shape) != (n,) or v.device != logits.device:
+            raise ValueError(f"{name} must be [{n}] on {logits.device}")
+    l, g = lse.to(acc).contiguous(), grad.to(acc).contiguous()
+    if out is None:
+        out = torch.empty(n, vocab, dtype=out_dtype or logits.dtype, device=logits.device)
+    elif (tuple(out.shape) != (n, vocab) or out.device != logits.device or out.dtype != (out_dtype or out.dtype)
+          or (vocab > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < vocab)):
+        raise ValueError(f"out must be [{n}, {vocab}] with dense rows on {logits.device}, of type {out_dtype}")
+    if out is not given and _overlap(out, logits):
+        raise ValueError("out may be the logits tensor itself, but not overlap it otherwise")
+    if out.dtype not in N.DTYPE_CODE:
+        raise ValueError(f"unsupported gradient dtype {out.dtype}")
+    with _on(logits):
+        rc = N.lib().kvs_distill_backward(logits.data_ptr(), _ld(logits), n, vocab, i.data_ptr(), t.data_ptr(),
+                                          i.shape[1], l.data_ptr(), g.data_ptr(), float(temperature),
+                                          N.DTYPE_CODE[logits.dtype], out.data_ptr(), _ld(out),
+                                          N.DTYPE_CODE[out.dtype], N.stream_ptr(logits.device))
+    N.check(rc, "kvs_distill_backward")
+    return out
+
+
+def _span(t: torch.Tensor):
+    last = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) if t.numel() else -1
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1

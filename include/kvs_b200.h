@@ -120,7 +120,8 @@ typedef struct kvs_batch {
 } kvs_batch;
 
 /* size of each public struct as compiled into the library (ABI check):
- * which = 0 kvs_cache, 1 kvs_batch, 2 kvs_decode_args, 3 kvs_replay_args, 4 kvs_segments */
+ * which = 0 kvs_cache, 1 kvs_batch, 2 kvs_decode_args, 3 kvs_replay_args, 4 kvs_segments,
+ * 5 kvs_linear_args, 6 kvs_linear_grads */
 size_t kvs_abi_struct_size(int which);
 int kvs_abi_version(void);
 /* number of SMs of the current device, cached per device (grid sizing) */
@@ -483,6 +484,82 @@ int kvs_silu_mul(const void* gu, void* out, int64_t n_rows, int32_t f, int64_t l
                  kvs_stream_t stream);
 int kvs_silu_mul_backward(const void* gu, const void* grad, void* dgu, int64_t n_rows, int32_t f, int64_t ld_gu,
                           int64_t ld_grad, int64_t ld_dgu, int32_t dtype, kvs_stream_t stream);
+
+/* ---------------------------------------------------------------- layer products
+ * The decoder layer's matrix products with their epilogues for half-precision models (KVS_BF16 /
+ * KVS_F16; model.py:58-63 and 74-75 the projections, model.py:78-86 the gated feed-forward, and
+ * the residual sums of model.py:149-152), one launch each, float32 accumulation, one rounding:
+ *   weight_up NULL:  out = act(x W^T + bias) + residual
+ *   weight_up given: out = act(x W^T) * (x W_up^T)            (no bias, no residual)
+ * x [rows][k], W and W_up [n][k] (a Linear layer's weight), bias [n], residual and out [rows][n];
+ * rows are ld_* elements apart.  pre (optional) receives the pre-activations for the backward:
+ * [rows][n], or [rows][2 n] = gate | up (the layout kvs_silu_mul reads).  out may be the residual.
+ * Any rows (0: nothing happens) and n; k and the pitches of x and the weights multiples of 8, their
+ * bases 16-byte aligned (KVS_E_UNSUPPORTED otherwise).  A bounded wait inside a kernel that runs
+ * out gives NaN outputs. */
+enum kvs_activation { KVS_ACT_NONE = 0, KVS_ACT_RELU = 1, KVS_ACT_SILU = 2, KVS_ACT_GELU = 3 /* erf form */ };
+typedef struct kvs_linear_args {
+  const void* x;
+  const void* weight;
+  const void* weight_up;
+  const void* bias;
+  const void* residual;
+  void* pre;
+  void* out;
+  int64_t ld_x;
+  int64_t ld_w;
+  int64_t ld_w_up;
+  int64_t ld_res;
+  int64_t ld_pre;
+  int64_t ld_out;
+  int32_t rows;
+  int32_t n;
+  int32_t k;
+  int32_t dtype;
+  int32_t activation;
+  int32_t reserved;
+} kvs_linear_args;
+int kvs_linear(const kvs_linear_args* a, kvs_stream_t stream);
+
+/* Gradients of kvs_linear for the upstream gradient gy [rows][n]; dx [rows][k], dw and dw_up [n][k],
+ * db [n], each written when its pointer is given (rows of dw and dw_up are ld_dw apart; gated needs
+ * dw and dw_up together and has no db).  a: x and the weights as in the forward, pre as the forward
+ * wrote it (needed when gated or with an activation); bias, residual and out are not read.  The
+ * gradient of the residual is gy itself.  Sums run in a fixed order (no float atomics).
+ * scratch: kvs_linear_backward_scratch_bytes(a, g) bytes, 256-byte aligned. */
+typedef struct kvs_linear_grads {
+  const void* gy;
+  void* dx;
+  void* dw;
+  void* dw_up;
+  void* db;
+  void* scratch;
+  size_t scratch_bytes;
+  int64_t ld_gy;
+  int64_t ld_dx;
+  int64_t ld_dw;
+} kvs_linear_grads;
+size_t kvs_linear_backward_scratch_bytes(const kvs_linear_args* a, const kvs_linear_grads* g);
+int kvs_linear_backward(const kvs_linear_args* a, const kvs_linear_grads* g, kvs_stream_t stream);
+
+/* Distillation from a teacher's top logits, beside kvs_lse_gather: row r of logits [n_rows][ld] has
+ * `top` slots ids[r][top], teacher[r][top] (dense; teacher in float, double for KVS_F64 logits; raw
+ * logits or log-probs, any shift).  A slot with id < 0, or a teacher value of -inf or NaN, is empty;
+ * with p = softmax(teacher[r] / T) over the kept slots,
+ *   lse[r]  = log sum_v exp(x[r][v] / T),
+ *   loss[r] = sum_kept p_j (log p_j - (x[r][id_j] / T - lse[r]))   (0 without kept slots)
+ * in float (double for KVS_F64).  dtype: any enum kvs_dtype.  An id may come twice.  A kept id
+ * >= vocab gives a NaN loss and gradient row.  top <= 1024 (KVS_E_UNSUPPORTED otherwise). */
+int kvs_distill(const void* logits, int64_t ld, int32_t n_rows, int32_t vocab, const int64_t* ids,
+                const void* teacher, int32_t top, double temperature, int32_t dtype, void* loss, void* lse,
+                kvs_stream_t stream);
+/* Its gradient with respect to the logits for upstream grad[r] (type of lse) with the forward's lse:
+ * dlogits[r][v] = grad[r] (exp(x[r][v]/T - lse[r]) - sum_{j: id_j = v} p_j) / T, zeros for a row
+ * without kept slots; in out_dtype (the logits' own, or KVS_BF16 / KVS_F16 from KVS_F32) with row
+ * stride ld_out.  dlogits may be the logits buffer itself when dtype and stride are its own. */
+int kvs_distill_backward(const void* logits, int64_t ld, int32_t n_rows, int32_t vocab, const int64_t* ids,
+                         const void* teacher, int32_t top, const void* lse, const void* grad, double temperature,
+                         int32_t dtype, void* dlogits, int64_t ld_out, int32_t out_dtype, kvs_stream_t stream);
 
 /* Self-test of the tcgen05 path (no reference counterpart): c[128][128] f32 =
  * a[128][128] (bf16 row-major) x B, with B given as bt[128 n][128 k] (mode bit 0 = 0,

@@ -1,0 +1,130 @@
+"""The layer products (kvs_linear / kvs_linear_backward, plain and gated) against float64 on the
+same half-precision inputs.
+
+Tolerances.  A forward output is a float32 sum of k exact products (a bf16 or fp16 product is exact
+in float32) plus bias, activation and residual, rounded once.  The sum's error is at most
+k * 2^-24 * sum|x w| and in practice far less: ACC = 2^-18 * sum|x||w| bounds it for k <= 4096 with
+rounding errors of either sign (64 ulps of the absolute sum), the activations add a few float32 ulps
+(covered by the same term) and the final rounding adds eps / 2 of the value.  A backward output is a
+sum of products of two rounded operands: dz carries half a step of its own (eps / 2) and, with an
+activation, the half step of the kept pre-activation times the activation's curvature, so each term
+is off by at most (eps / 2)(1 + C) relative to gy's scale; the bound is that share of the absolute
+sum.  The absolute sums are computed in float64 beside the result."""
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+pytestmark = pytest.mark.gpu
+
+ACT = {None: lambda z: z, "relu": torch.relu, "silu": F.silu, "gelu": F.gelu}
+# largest |act'| and |act''| (silu 1.10 / 0.5, gelu 1.13 / 0.80 = 2 phi(0)); a pre-activation off by
+# delta changes act' by at most curv * delta.  relu's derivative jumps at 0, which a rounding to
+# nearest never crosses: a sum of the other sign would have to be below the smallest subnormal.
+SLOPE = {None: (1.0, 0.0), "relu": (1.0, 0.0), "silu": (1.1, 0.5), "gelu": (1.13, 0.8)}
+ACC = 2.0 ** -18
+
+
+def _half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _rand(g, *shape, scale=1.0, dtype=torch.bfloat16):
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def _near(got, want, bound, dtype, what):
+    """|got - want| <= half a step of want + bound (+ the smallest subnormal of the type)."""
+    tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    err = (got.double() - want).abs() - (want.abs() * _half(dtype) * 1.01 + bound + tiny)
+    assert err.max().item() <= 0, (what, err.max().item())
+
+
+SIZES = [(1, 1, 8), (1, 4096, 512), (3, 129, 72), (64, 256, 64), (130, 255, 136), (257, 513, 200), (300, 1000, 1032),
+         (777, 130, 4096)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", [None, "relu", "silu", "gelu"])
+@pytest.mark.parametrize("rows,n,k", SIZES)
+def test_linear_forward(rows, n, k, act, dtype):
+    from kvstreams import ops
+
+    g = torch.Generator(device="cuda").manual_seed(rows * 7 + n + k)
+    x, w, b, r = _rand(g, rows, k, dtype=dtype), _rand(g, n, k, scale=0.1, dtype=dtype), _rand(g, n, dtype=dtype), _rand(g, rows, n, dtype=dtype)
+    z0 = x.double() @ w.double().t()
+    mass = (x.double().abs() @ w.double().abs().t()) * ACC
+    for bias, res in ((None, None), (b, r)):
+        pre = ops.pre_buffer(x, n)
+        y = ops.linear(x, w, bias=bias, residual=res, activation=act, pre=pre)
+        z = z0 if bias is None else z0 + bias.double()
+        want = ACT[act](z) if res is None else ACT[act](z) + res.double()
+        extra = mass * 2 + (z.abs() + 1) * 2.0 ** -20
+        _near(pre, z, extra, dtype, "pre")
+        _near(y, want, extra, dtype, "y")
+        assert torch.equal(y, ops.linear(x, w, bias=bias, residual=res, activation=act))  # pre changes nothing
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", [None, "relu", "silu", "gelu"])
+@pytest.mark.parametrize("rows,n,k", SIZES)
+def test_linear_backward(rows, n, k, act, dtype):
+    from kvstreams import ops
+
+    g = torch.Generator(device="cuda").manual_seed(rows * 5 + n + k)
+    x, w, b, gy = _rand(g, rows, k, dtype=dtype), _rand(g, n, k, scale=0.1, dtype=dtype), _rand(g, n, dtype=dtype), _rand(g, rows, n, dtype=dtype)
+    pre = ops.pre_buffer(x, n)
+    ops.linear(x, w, bias=b, activation=act, pre=pre)
+    dx, dw, db = ops.linear_backward(gy, x, w, pre=pre, activation=act, bias_grad=True)
+    xd, wd, bd = (t.double().requires_grad_() for t in (x, w, b))
+    z = F.linear(xd, wd, bd)
+    want = torch.autograd.grad(ACT[act](z), [xd, wd, bd], gy.double())
+    # the derivative is taken at the kept pre-activation, half a step from z
+    slope, curv = SLOPE[act]
+    h = _half(dtype)
+    off = gy.double().abs() * (curv * (z.detach().abs() * h + 2.0 ** -16) + slope * (h + 2.0 ** -20))
+    if act == "relu":  # z of either sign within the float32 sum's error of 0 may take either derivative
+        off = off + gy.double().abs() * (z.detach().abs() < 2.0 ** -12)
+    big = gy.double().abs() * slope
+    _near(dx, want[0], off @ w.double().abs() + big @ w.double().abs() * ACC, dtype, "dx")
+    _near(dw, want[1], off.t() @ x.double().abs() + big.t() @ x.double().abs() * ACC, dtype, "dw")
+    _near(db, want[2], off.sum(0) + big.sum(0) * ACC, dtype, "db")
+    again = ops.linear_backward(gy, x, w, pre=pre, activation=act, bias_grad=True)
+    assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), again))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu", None])
+@pytest.mark.parametrize("rows,n,k", SIZES)
+def test_gated_linear(rows, n, k, act, dtype):
+    from kvstreams import ops
+
+    g = torch.Generator(device="cuda").manual_seed(rows * 3 + n + k)
+    x, gh = _rand(g, rows, k, dtype=dtype), _rand(g, rows, n, dtype=dtype)
+    wg, wu = _rand(g, n, k, scale=0.05, dtype=dtype), _rand(g, n, k, scale=0.05, dtype=dtype)
+    pre = ops.pre_buffer(x, 2 * n)
+    h = ops.gated_linear(x, wg, wu, activation=act, pre=pre)
+    dx, dwg, dwu = ops.gated_linear_backward(gh, x, wg, wu, pre, activation=act)
+    xd, gd, ud = (t.double().requires_grad_() for t in (x, wg, wu))
+    zg, zu = F.linear(xd, gd), F.linear(xd, ud)
+    y = ACT[act](zg) * zu
+    want = torch.autograd.grad(y, [xd, gd, ud], gh.double())
+    zg, zu, y = zg.detach(), zu.detach(), y.detach()
+    ax, ag, au = x.double().abs(), wg.double().abs(), wu.double().abs()
+    mg, mu = ax @ ag.t() * ACC + 2.0 ** -20, ax @ au.t() * ACC + 2.0 ** -20  # float32 errors of g, u
+    slope, curv = SLOPE[act]
+    _near(pre[:, :n], zg, mg, dtype, "gate")
+    _near(pre[:, n:], zu, mu, dtype, "up")
+    _near(h, y, slope * mg * (zu.abs() + mu) + (zg.abs() * slope + mg) * mu + y.abs() * 2.0 ** -20, dtype, "h")
+    assert torch.equal(h, ops.gated_linear(x, wg, wu, activation=act))
+    hs = _half(dtype)
+    eg, eu = zg.abs() * hs + mg, zu.abs() * hs + mu  # how far the kept g, u are off
+    gm = gh.double().abs()
+    # dg = gh u act'(g): off by gh (eu slope + |u| curv eg), rounded (hs); du = gh act(g) likewise
+    jump = (zg.abs() < 2.0 ** -12).double() if act == "relu" else 0.0
+    og = gm * (eu * slope + (zu.abs() + eu) * (curv * eg + jump + slope * (hs + 2.0 ** -20)))
+    ou = gm * (slope * eg + (zg.abs() + eg) * slope * (hs + 2.0 ** -20))
+    bg, bu = gm * (zu.abs() * slope + 1), gm * (zg.abs() * slope + 1)
+    _near(dx, want[0], og @ ag + ou @ au + (bg @ ag + bu @ au) * ACC, dtype, "dx")
+    _near(dwg, want[1], (og.t() + bg.t() * ACC) @ ax, dtype, "dwg")
+    _near(dwu, want[2], (ou.t() + bu.t() * ACC) @ ax, dtype, "dwu")
