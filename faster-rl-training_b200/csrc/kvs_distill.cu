@@ -11,11 +11,18 @@
 //
 // Bound by HBM: the forward reads each logits row once, the backward reads it once and writes
 // the gradient once (nothing is read for a row without kept slots).
+//
+// A group of G threads takes a row (or a segment of one): a whole CTA of 256 usually, a warp for
+// short rows, where a CTA's barriers would cost more than the row.  When there are too few rows
+// to fill the machine, the CTAs of a row (a cluster in the forward, which joins their maxima and
+// sums through distributed shared memory) take contiguous segments of it.
 #include <algorithm>
 #include <cmath>
+#include <cooperative_groups.h>
 #include <type_traits>
 
 #include "kvs_common.cuh"
+#include "kvs_sm100.cuh"
 
 using namespace kvs;
 
@@ -23,104 +30,218 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTop = 1024;
+constexpr int kWarpTop = 128;      // slots of a row that a warp takes
+constexpr int kMaxSegments = 8;    // CTAs of one row
 
-__device__ __forceinline__ float exp_of(float x) { return __expf(x); }
-__device__ __forceinline__ double exp_of(double x) { return exp(x); }
 __device__ __forceinline__ float exp_full(float x) { return expf(x); }
 __device__ __forceinline__ double exp_full(double x) { return exp(x); }
 __device__ __forceinline__ float log_full(float x) { return logf(x); }
 __device__ __forceinline__ double log_full(double x) { return log(x); }
+// exp(d / T) with c = log2(e) / T for float, 1 / T for double.  The hardware's 2^x (2^-22 relative;
+// results below 2^-126, which no sum or rounded gradient here can tell from 0, become 0).
+__device__ __forceinline__ float exp_scaled(float d, float c) { return sm100::ex2_approx(d * c); }
+__device__ __forceinline__ double exp_scaled(double d, double c) { return exp(d * c); }
 
-template <typename A> __device__ __forceinline__ A block_sum(A v, A* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  A r = A(0);
-  for (int i = 0; i < kThreads / 32; ++i) r += red[i];
-  __syncthreads();
-  return r;
+template <int G> __device__ __forceinline__ void group_sync() {
+  if constexpr (G == 32) __syncwarp();
+  else __syncthreads();
 }
-template <typename A> __device__ __forceinline__ A block_max(A v, A* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const A w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = w > v ? w : v;
-  }
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  A r = -INFINITY;
-  for (int i = 0; i < kThreads / 32; ++i) r = red[i] > r ? red[i] : r;
-  __syncthreads();
-  return r;
-}
-
-// The teacher's softmax statistics of one row (all threads of the CTA): the largest kept t_j,
-// sum exp((t_j - max) / T) over the kept slots, and whether a kept id is past the vocabulary.
-template <typename A>
-struct Teacher {
-  A m, z;
-  bool any, bad;
+struct MaxOp {
+  template <typename A> __device__ A operator()(A a, A b) const { return b > a ? b : a; }
 };
-template <typename A>
-__device__ Teacher<A> teacher_stats(const int64_t* ids, const A* t, int top, int vocab, A inv_temp, A* red) {
-  A m = -INFINITY;
-  int bad = 0;
-  for (int j = threadIdx.x; j < top; j += kThreads) {
-    if (ids[j] >= 0 && t[j] > -INFINITY) {
-      m = t[j] > m ? t[j] : m;
-      bad |= ids[j] >= vocab;
-    }
+struct SumOp {
+  template <typename A> __device__ A operator()(A a, A b) const { return a + b; }
+};
+// N values reduced over the group at once (one pair of barriers); `red`: N per warp of the CTA
+template <int G, typename Op, typename A, int N> __device__ __forceinline__ void group_reduce(A (&v)[N], A* red) {
+  const Op op;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = op(v[k], __shfl_xor_sync(0xffffffffu, v[k], o));
+  if constexpr (G != 32) {
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int k = 0; k < N; ++k) red[(threadIdx.x >> 5) * N + k] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = red[k];
+#pragma unroll
+    for (int i = 1; i < G / 32; ++i)
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] = op(v[k], red[i * N + k]);
+    __syncthreads();
   }
-  Teacher<A> r;
-  r.m = block_max(m, red);
-  r.any = r.m > -INFINITY;
-  r.bad = __syncthreads_or(bad) != 0;
-  A z = A(0);
-  for (int j = threadIdx.x; j < top; j += kThreads)
-    if (ids[j] >= 0 && t[j] > -INFINITY) z += exp_full((t[j] - r.m) * inv_temp);
-  r.z = block_sum(z, red);
-  return r;
 }
 
-// one CTA per row
-template <typename T, typename A>
-__global__ void __launch_bounds__(kThreads)
-distill_kernel(const T* __restrict__ logits, int64_t ld, int vocab, const int64_t* __restrict__ ids,
-               const A* __restrict__ teacher, int top, A inv_temp, A* __restrict__ loss, A* __restrict__ lse_out) {
-  __shared__ A red[kThreads / 32];
-  const int64_t row = blockIdx.x;
-  const T* x = logits + row * ld;
-  A m = -INFINITY, s = A(0);
-  for (int i = threadIdx.x; i < vocab; i += kThreads) {
-    const A v = to_acc<T>(x[i]) * inv_temp;
+// A thread's slots of a row, in registers: loaded before the row is streamed, so that their
+// latency is behind it.  id < 0: empty.
+template <typename A, int PER>
+struct Slots {
+  int64_t id[PER];
+  A t[PER];
+};
+template <int G, typename A, int PER>
+__device__ __forceinline__ void load_slots(const int64_t* ids, const A* t, int top, int tid, Slots<A, PER>& s) {
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int j = tid + u * G;
+    s.id[u] = -1;
+    s.t[u] = -INFINITY;
+    if (j < top) {
+      s.id[u] = ids[j];
+      s.t[u] = t[j];
+    }
+    if (!(s.t[u] > -INFINITY)) s.id[u] = -1;
+  }
+}
+
+// 16 bytes of a row
+template <typename T> struct alignas(16) Pack {
+  static constexpr int n = 16 / sizeof(T);
+  T v[n];
+};
+
+// elements before the first 16-byte boundary of `p`, at most `n`
+template <typename T> __device__ __forceinline__ int head_of(const T* p, int n) {
+  const int h = (int)(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T));
+  return min(h, n);
+}
+
+// Running (max, sum of exp((x - max) / T)) of a thread's share of `n` elements at x: 16-byte loads
+// between the ends, kUnroll of them in flight, one rescale of the sum per batch.
+template <int G, typename T, typename A>
+__device__ void row_lse(const T* __restrict__ x, int n, A c, int tid, A& m, A& s) {
+  using P = Pack<T>;
+  constexpr int kUnroll = 4;
+  auto one = [&](T e) {
+    const A v = to_acc<T>(e);
     if (v > m) {
-      s = s * exp_of(m - v) + A(1);
+      s = s * exp_scaled(m - v, c) + A(1);
       m = v;
-    } else if (v != -INFINITY) {
-      s += exp_of(v - m);
+    } else if (v != -INFINITY) {  // (-inf - -inf has no exponential; it adds nothing)
+      s += exp_scaled(v - m, c);
+    }
+  };
+  const int head = head_of(x, n);
+  const int packs = (n - head) / P::n;
+  const P* xp = reinterpret_cast<const P*>(x + head);
+  if (tid < head) one(x[tid]);
+  const int tail = head + packs * P::n + tid;
+  if (tail < n) one(x[tail]);  // fewer than P::n <= G elements
+  for (int i0 = tid; i0 < packs; i0 += kUnroll * G) {
+    P q[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (i0 + u * G < packs) *reinterpret_cast<uint4*>(&q[u]) = __ldg(reinterpret_cast<const uint4*>(xp + i0 + u * G));
+    A bm = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (i0 + u * G < packs) {
+#pragma unroll
+        for (int k = 0; k < P::n; ++k) {
+          const A v = to_acc<T>(q[u].v[k]);
+          bm = v > bm ? v : bm;
+        }
+      }
+    if (bm > m) {
+      s *= exp_scaled(m - bm, c);
+      m = bm;
+    }
+    // while nothing but -inf came, a reference of 0 keeps the differences away from inf - inf
+    const A ref = m == -INFINITY ? A(0) : m;
+    A part = A(0);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (i0 + u * G < packs) {
+#pragma unroll
+        for (int k = 0; k < P::n; ++k) part += exp_scaled(to_acc<T>(q[u].v[k]) - ref, c);
+      }
+    s += part;
+  }
+}
+
+// Grid: rows / (256 / G) CTAs of one row group each, times `segs` CTAs (one cluster) per row.
+template <typename T, typename A, int G>
+__global__ void __launch_bounds__(kThreads)
+distill_kernel(const T* __restrict__ logits, int64_t ld, int n_rows, int vocab, const int64_t* __restrict__ ids,
+               const A* __restrict__ teacher, int top, A inv_temp, A c, int segs, A* __restrict__ loss,
+               A* __restrict__ lse_out) {
+  constexpr int PER = (G == 32 ? kWarpTop : kMaxTop) / G;
+  __shared__ A red[3 * (kThreads / 32)];
+  __shared__ A part[2];
+  const int tid = threadIdx.x % G;
+  const int seg = segs > 1 ? (int)(blockIdx.x % segs) : 0;
+  const int64_t row = (int64_t)(blockIdx.x / segs) * (kThreads / G) + threadIdx.x / G;
+  if (G == 32 && row >= n_rows) return;
+  const T* x = logits + row * ld;
+  int beg = 0, len = vocab;
+  if (segs > 1) {
+    const int per = (vocab + segs - 1) / segs;
+    beg = min(seg * per, vocab);
+    len = min(per, vocab - beg);
+  }
+  Slots<A, PER> slot;
+  load_slots<G>(ids + row * top, teacher + row * top, seg == 0 ? top : 0, tid, slot);
+  T xs[PER];
+  A bad = A(0), tm = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    xs[u] = T(0.f);
+    if (slot.id[u] >= 0) {
+      tm = slot.t[u] > tm ? slot.t[u] : tm;
+      if (slot.id[u] < vocab) xs[u] = x[slot.id[u]];
+      else bad = A(1);
     }
   }
-  const A mm = block_max(m, red);
-  // a thread that saw only -inf adds nothing (its exponent would be inf - inf)
-  const A S = block_sum(m == -INFINITY && s == A(0) ? A(0) : s * exp_full(m - mm), red);
-  const A lse = mm + log_full(S);
-  const int64_t* id = ids + row * top;
-  const A* t = teacher + row * top;
-  const Teacher<A> te = teacher_stats(id, t, top, vocab, inv_temp, red);
-  A part = A(0);
-  if (te.any && !te.bad) {
-    const A logz = log_full(te.z);
-    for (int j = threadIdx.x; j < top; j += kThreads) {
-      if (!(id[j] >= 0 && t[j] > -INFINITY)) continue;
-      const A lp = (t[j] - te.m) * inv_temp - logz;
-      const A p = exp_full(lp);
-      if (p != A(0)) part += p * (lp - (to_acc<T>(x[id[j]]) * inv_temp - lse));
-    }
+  A m = -INFINITY, s = A(0);
+  row_lse<G, T, A>(x + beg, len, c, tid, m, s);
+  A mx[2] = {m, tm};
+  group_reduce<G, MaxOp>(mx, red);
+  tm = mx[1];
+  // a thread that saw nothing but -inf has s == 0 and adds nothing; a NaN stays one
+  A sum[3] = {s == A(0) ? A(0) : s * exp_scaled(m - mx[0], c), A(0), bad};
+  A e[PER];
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    e[u] = slot.id[u] >= 0 ? (slot.t[u] - tm) * inv_temp : A(0);  // log of the weight times their sum
+    if (slot.id[u] >= 0) sum[1] += exp_full(e[u]);
   }
-  const A l = block_sum(part, red);
-  if (threadIdx.x == 0) {
-    loss[row] = te.bad ? A(NAN) : l;
+  group_reduce<G, SumOp>(sum, red);
+  A mm = mx[0], S = sum[0];
+  if (segs > 1) {  // join the segments in order; the first CTA of the cluster goes on
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    if (threadIdx.x == 0) {
+      part[0] = mm;
+      part[1] = S;
+    }
+    cluster.sync();
+    if (seg == 0) {  // every thread reads the few pairs: no further exchange
+      A all = -INFINITY, tot = A(0);
+      for (int i = 0; i < segs; ++i) all = MaxOp()(all, cluster.map_shared_rank(part, i)[0]);
+      for (int i = 0; i < segs; ++i) {
+        const A* r = cluster.map_shared_rank(part, i);
+        if (r[1] != A(0)) tot += r[1] * exp_scaled(r[0] - all, c);
+      }
+      mm = all;
+      S = tot;
+    }
+    cluster.sync();  // the others' shared memory stays until it is read
+    if (seg != 0) return;
+  }
+  const A lse = mm * inv_temp + log_full(S);
+  const A logz = log_full(sum[1]);
+  A term[1] = {A(0)};
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    if (slot.id[u] < 0) continue;
+    const A lp = e[u] - logz, p = exp_full(lp);
+    if (p != A(0)) term[0] += p * (lp - (to_acc<T>(xs[u]) * inv_temp - lse));
+  }
+  group_reduce<G, SumOp>(term, red);
+  if (tid == 0) {
+    loss[row] = sum[2] > A(0) ? A(NAN) : term[0];
     lse_out[row] = lse;
   }
 }
@@ -131,42 +252,96 @@ template <typename O, typename A> __device__ __forceinline__ O round_to(A v) {
   else return (O)v;
 }
 
-// one CTA per row; dlogits may be the logits themselves
-template <typename T, typename A, typename O>
+// N values to d, as widely as d's address allows
+template <typename O, typename A, int N> __device__ __forceinline__ void put(O* d, const A (&v)[N]) {
+  struct alignas(sizeof(O) * N > 16 ? 16 : sizeof(O) * N) Out { O v[N]; } o;
+#pragma unroll
+  for (int k = 0; k < N; ++k) o.v[k] = round_to<O, A>(v[k]);
+  if ((reinterpret_cast<uintptr_t>(d) & (alignof(Out) - 1)) == 0) {
+    *reinterpret_cast<Out*>(d) = o;
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) d[k] = o.v[k];
+  }
+}
+
+// dlogits may be the logits themselves.  A CTA writes only its segment, after it has read what it
+// needs of it (the entries that slots name).
+template <typename T, typename A, typename O, int G>
 __global__ void __launch_bounds__(kThreads)
-distill_bwd_kernel(const T* logits, int64_t ld, int vocab, const int64_t* __restrict__ ids,
+distill_bwd_kernel(const T* logits, int64_t ld, int n_rows, int vocab, const int64_t* __restrict__ ids,
                    const A* __restrict__ teacher, int top, const A* __restrict__ lse_in, const A* __restrict__ grad,
-                   A inv_temp, O* dlogits, int64_t ld_out) {
-  __shared__ A red[kThreads / 32];
-  __shared__ A sp[kMaxTop];
-  __shared__ int sid[kMaxTop];
-  const int64_t row = blockIdx.x;
+                   A inv_temp, A c, int segs, O* dlogits, int64_t ld_out) {
+  constexpr int TOP = G == 32 ? kWarpTop : kMaxTop, PER = TOP / G;
+  __shared__ A red[2 * (kThreads / 32)];
+  __shared__ A sp_all[kThreads / G][TOP];
+  __shared__ int sid_all[kThreads / G][TOP];
+  const int tid = threadIdx.x % G, group = threadIdx.x / G;
+  A* sp = sp_all[group];
+  int* sid = sid_all[group];
+  const int seg = segs > 1 ? (int)(blockIdx.x % segs) : 0;
+  const int64_t row = (int64_t)(blockIdx.x / segs) * (kThreads / G) + group;
+  if (G == 32 && row >= n_rows) return;
+  int beg = 0, len = vocab;
+  if (segs > 1) {
+    const int per = (vocab + segs - 1) / segs;
+    beg = min(seg * per, vocab);
+    len = min(per, vocab - beg);
+  }
   const T* x = logits + row * ld;
   O* d = dlogits + row * ld_out;
-  const int64_t* id = ids + row * top;
-  const A* t = teacher + row * top;
-  const Teacher<A> te = teacher_stats(id, t, top, vocab, inv_temp, red);
-  if (!te.any || te.bad) {
-    const O fill = round_to<O, A>(te.bad ? A(NAN) : A(0));
-    for (int i = threadIdx.x; i < vocab; i += kThreads) d[i] = fill;
+  const A lse = lse_in[row], g = grad[row] * inv_temp;
+  // exp(x / T - lse) = exp((x - lse T) / T): the difference is formed before it is scaled
+  const A at_one = lse / inv_temp;
+  auto prob = [&](T e) { return g * exp_scaled(to_acc<T>(e) - at_one, c); };
+  Slots<A, PER> slot;
+  load_slots<G>(ids + row * top, teacher + row * top, top, tid, slot);
+  T xs[PER];
+  A tm[1] = {-INFINITY}, sum[2] = {A(0), A(0)};
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    xs[u] = T(0.f);
+    if (slot.id[u] >= vocab) sum[1] = A(1);
+    if (slot.id[u] >= beg && slot.id[u] < beg + len) xs[u] = x[slot.id[u]];
+    tm[0] = slot.id[u] >= 0 ? MaxOp()(tm[0], slot.t[u]) : tm[0];
+  }
+  group_reduce<G, MaxOp>(tm, red);
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    slot.t[u] = slot.id[u] >= 0 ? exp_full((slot.t[u] - tm[0]) * inv_temp) : A(0);
+    sum[0] += slot.t[u];
+    const int j = tid + u * G;
+    if (j < top) {
+      sid[j] = slot.id[u] < 0 ? -1 : (int)slot.id[u];
+      sp[j] = slot.t[u];
+    }
+  }
+  group_reduce<G, SumOp>(sum, red);
+  if constexpr (G == 32) __syncwarp();
+  using P = Pack<T>;
+  const int head = head_of(x + beg, len);
+  const int packs = (len - head) / P::n;
+  const bool bad = sum[1] > A(0);
+  if (!(tm[0] > -INFINITY) || bad) {
+    const A one = bad ? A(NAN) : A(0);
+    A v[P::n];
+#pragma unroll
+    for (int k = 0; k < P::n; ++k) v[k] = one;
+    O* dp = d + beg + head;
+    if (tid < head) d[beg + tid] = round_to<O, A>(one);
+    for (int i = tid; i < packs; i += G) put<O, A, P::n>(dp + (int64_t)i * P::n, v);
+    for (int i = head + packs * P::n + tid; i < len; i += G) d[beg + i] = round_to<O, A>(one);
     return;
   }
-  const A lse = lse_in[row], g = grad[row] * inv_temp, inv_z = A(1) / te.z;
-  for (int j = threadIdx.x; j < top; j += kThreads) {
-    const bool keep = id[j] >= 0 && t[j] > -INFINITY;
-    sid[j] = keep ? (int)id[j] : -1;
-    sp[j] = keep ? exp_full((t[j] - te.m) * inv_temp) * inv_z : A(0);
-  }
-  __syncthreads();
-  // the entries that a slot names, before the row is overwritten: the first slot of an id takes
-  // the sum of all its slots, in slot order
-  constexpr int PER = kMaxTop / kThreads;
+  // the first slot of an id takes the sum of all its slots, in slot order
+  const A gz = g / sum[0];
   A val[PER];
   int at[PER];
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
-    const int j = threadIdx.x + u * kThreads;
-    at[u] = j < top ? sid[j] : -1;
+    const int j = tid + u * G;
+    at[u] = (int)slot.id[u];
+    if (slot.id[u] < beg || slot.id[u] >= beg + len) at[u] = -1;
     if (at[u] >= 0) {
       A p = A(0);
       for (int i = 0; i < top; ++i) {
@@ -177,24 +352,84 @@ distill_bwd_kernel(const T* logits, int64_t ld, int vocab, const int64_t* __rest
         }
         p += sp[i];
       }
-      if (at[u] >= 0) val[u] = g * (exp_of(to_acc<T>(x[at[u]]) * inv_temp - lse) - p);
+      if (at[u] >= 0) val[u] = prob(xs[u]) - gz * p;
     }
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < vocab; i += kThreads)
-    d[i] = round_to<O, A>(g * exp_of(to_acc<T>(x[i]) * inv_temp - lse));
-  __syncthreads();
+  // (every slot's logit was read before the first barrier above)
+  {
+    constexpr int kUnroll = 4;
+    const P* xp = reinterpret_cast<const P*>(x + beg + head);
+    O* dp = d + beg + head;
+    if (tid < head) d[beg + tid] = round_to<O, A>(prob(x[beg + tid]));
+    for (int i = head + packs * P::n + tid; i < len; i += G) d[beg + i] = round_to<O, A>(prob(x[beg + i]));
+    for (int i0 = tid; i0 < packs; i0 += kUnroll * G) {
+      P q[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (i0 + u * G < packs) *reinterpret_cast<uint4*>(&q[u]) = *reinterpret_cast<const uint4*>(xp + i0 + u * G);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (i0 + u * G < packs) {
+          A v[P::n];
+#pragma unroll
+          for (int k = 0; k < P::n; ++k) v[k] = prob(q[u].v[k]);
+          put<O, A, P::n>(dp + (int64_t)(i0 + u * G) * P::n, v);
+        }
+    }
+  }
+  group_sync<G>();
 #pragma unroll
   for (int u = 0; u < PER; ++u)
     if (at[u] >= 0) d[at[u]] = round_to<O, A>(val[u]);
 }
 
+// Short rows go to warps: below this many bytes a row's own work is shorter than a CTA's barriers.
+constexpr int kWarpRowBytes = 4096;
+template <typename T> bool warp_rows(int vocab, int top, int n_rows) {
+  return (int64_t)vocab * (int64_t)sizeof(T) <= kWarpRowBytes && top <= kWarpTop;
+}
+// CTAs per row: doubled while the rows give the machine less than eight CTAs an SM and a segment
+// keeps 8 KB (two 16-byte loads a thread)
+template <typename T> int segments(int vocab, int n_rows) {
+  int s = 1;
+  while (s < kMaxSegments && (int64_t)n_rows * s < 4 * 148 && (int64_t)vocab * (int64_t)sizeof(T) / (2 * s) >= 8192)
+    s *= 2;
+  return s;
+}
+template <typename A> A log2e_of(double inv_temp) {
+  return (A)(std::is_same<A, double>::value ? inv_temp : inv_temp * 1.4426950408889634);
+}
+
 template <typename T, typename A>
 int launch_fwd(const void* logits, int64_t ld, int32_t n_rows, int32_t vocab, const int64_t* ids, const void* teacher,
                int32_t top, double temperature, void* loss, void* lse, cudaStream_t st) {
-  distill_kernel<T, A><<<(unsigned)n_rows, kThreads, 0, st>>>(
-      static_cast<const T*>(logits), ld, vocab, ids, static_cast<const A*>(teacher), top, (A)(1.0 / temperature),
-      static_cast<A*>(loss), static_cast<A*>(lse));
+  const T* x = static_cast<const T*>(logits);
+  const A* t = static_cast<const A*>(teacher);
+  const A inv = (A)(1.0 / temperature), c = log2e_of<A>(1.0 / temperature);
+  A *l = static_cast<A*>(loss), *e = static_cast<A*>(lse);
+  if (warp_rows<T>(vocab, top, n_rows)) {
+    constexpr int R = kThreads / 32;
+    distill_kernel<T, A, 32><<<(n_rows + R - 1) / R, kThreads, 0, st>>>(x, ld, n_rows, vocab, ids, t, top, inv, c, 1,
+                                                                       l, e);
+    return launch_rc();
+  }
+  const int segs = segments<T>(vocab, n_rows);
+  if (segs == 1) {
+    distill_kernel<T, A, kThreads><<<n_rows, kThreads, 0, st>>>(x, ld, n_rows, vocab, ids, t, top, inv, c, 1, l, e);
+    return launch_rc();
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(n_rows * segs);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = segs;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, distill_kernel<T, A, kThreads>, x, ld, (int)n_rows, (int)vocab, ids, t, (int)top, inv, c,
+                     segs, l, e);
   return launch_rc();
 }
 
@@ -202,10 +437,19 @@ template <typename T, typename A, typename O>
 int launch_bwd(const void* logits, int64_t ld, int32_t n_rows, int32_t vocab, const int64_t* ids, const void* teacher,
                int32_t top, const void* lse, const void* grad, double temperature, void* dlogits, int64_t ld_out,
                cudaStream_t st) {
-  distill_bwd_kernel<T, A, O><<<(unsigned)n_rows, kThreads, 0, st>>>(
-      static_cast<const T*>(logits), ld, vocab, ids, static_cast<const A*>(teacher), top,
-      static_cast<const A*>(lse), static_cast<const A*>(grad), (A)(1.0 / temperature), static_cast<O*>(dlogits),
-      ld_out);
+  const T* x = static_cast<const T*>(logits);
+  const A *t = static_cast<const A*>(teacher), *e = static_cast<const A*>(lse), *g = static_cast<const A*>(grad);
+  const A inv = (A)(1.0 / temperature), c = log2e_of<A>(1.0 / temperature);
+  O* d = static_cast<O*>(dlogits);
+  if (warp_rows<T>(vocab, top, n_rows)) {
+    constexpr int R = kThreads / 32;
+    distill_bwd_kernel<T, A, O, 32><<<(n_rows + R - 1) / R, kThreads, 0, st>>>(x, ld, n_rows, vocab, ids, t, top, e, g,
+                                                                              inv, c, 1, d, ld_out);
+  } else {
+    const int segs = segments<T>(vocab, n_rows);
+    distill_bwd_kernel<T, A, O, kThreads><<<n_rows * segs, kThreads, 0, st>>>(x, ld, n_rows, vocab, ids, t, top, e, g,
+                                                                             inv, c, segs, d, ld_out);
+  }
   return launch_rc();
 }
 

@@ -8,9 +8,10 @@
 //                       dWg = dg^T x,  dWu = du^T x
 //
 // Every product accumulates in float32 (TMEM); bias, activation, gate product and residual are
-// applied to the float32 sums and the result is rounded once.  Two roundings lie inside: the
-// pre-activations kept for the backward (`pre`) and dz / dg / du, which are operands of the
-// tensor cores, have the activations' type (half a step, 2^-9 relative for bf16, each).
+// applied to the float32 sums and the result is rounded once.  One rounding lies inside: dz / dg /
+// du, operands of the tensor cores, have the activations' type (half a step, 2^-9 relative for
+// bf16).  The pre-activations kept for the backward (`pre`) are float32, or, where the caller
+// prefers half the memory to another rounding of that size, of the activations' type.
 //
 // pair_gemm_kernel: units of 256 rows x 256 columns of the result, computed by a pair of CTAs
 // (a 2-CTA cluster) with M = 256 tcgen05 MMAs (cta_group::2).  Each CTA stages its 128 rows of
@@ -22,8 +23,8 @@
 // even CTA stages rows of Wg and the odd one rows of Wu, and a thread of the epilogue finds
 // g and u of one output in the same TMEM lane.
 //
-// Roles per CTA (256 threads): warp 0 lane 0 = TMA producer (6-stage ring of 32 KB), warp 1 =
-// TMEM allocation and, in the even CTA, the MMA issuer; warps 4..7 = epilogue.  TMEM holds two
+// Roles per CTA (384 threads): warp 0 lane 0 = TMA producer (6-stage ring of 32 KB), warp 1 =
+// TMEM allocation and, in the even CTA, the MMA issuer; warps 4..11 = epilogue.  TMEM holds two
 // 256-column accumulators, so the epilogue of one unit overlaps the MMAs of the next.  Persistent
 // grid: pair p takes units p, p + P, ...  Every wait is bounded; after one that ran out the
 // outputs of the units concerned are NaN.
@@ -68,38 +69,35 @@ __device__ __forceinline__ void act_grad_f(float z, int act, float& a, float& da
   }
 }
 
-template <typename T> struct alignas(8) Vec4 { T v[4]; };
+template <typename T> struct alignas(sizeof(T) * 4) Vec4 { T v[4]; };
 template <typename T> struct alignas(16) Vec8 { T v[8]; };
 
-// four consecutive elements, `n` of them existing; one 8-byte access when `vec`
-template <typename T>
-__device__ __forceinline__ float4 load4(const T* p, int n, bool vec) {
-  float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (vec && n >= 4) {
-    const Vec4<T> q = *reinterpret_cast<const Vec4<T>*>(p);
-    r = make_float4(to_acc<T>(q.v[0]), to_acc<T>(q.v[1]), to_acc<T>(q.v[2]), to_acc<T>(q.v[3]));
-  } else {
-    if (n > 0) r.x = to_acc<T>(p[0]);
-    if (n > 1) r.y = to_acc<T>(p[1]);
-    if (n > 2) r.z = to_acc<T>(p[2]);
-    if (n > 3) r.w = to_acc<T>(p[3]);
-  }
-  return r;
+// four consecutive elements in one access
+template <typename T> __device__ __forceinline__ float4 load4(const T* p) {
+  const Vec4<T> q = *reinterpret_cast<const Vec4<T>*>(p);
+  return make_float4(to_acc<T>(q.v[0]), to_acc<T>(q.v[1]), to_acc<T>(q.v[2]), to_acc<T>(q.v[3]));
 }
-template <typename T>
-__device__ __forceinline__ void store4(T* p, float4 f, int n, bool vec) {
+template <typename T> __device__ __forceinline__ void store4(T* p, float4 f) {
   Vec4<T> q;
   q.v[0] = from_acc<T>(f.x);
   q.v[1] = from_acc<T>(f.y);
   q.v[2] = from_acc<T>(f.z);
   q.v[3] = from_acc<T>(f.w);
-  if (vec && n >= 4) {
-    *reinterpret_cast<Vec4<T>*>(p) = q;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) p[i] = q.v[i];
-  }
+  *reinterpret_cast<Vec4<T>*>(p) = q;
+}
+template <typename T> __device__ __forceinline__ void store_pre(void* pre, int64_t i, float4 f, bool f32) {
+  if (f32) store4(static_cast<float*>(pre) + i, f);
+  else store4(static_cast<T*>(pre) + i, f);
+}
+// a running pointer the compiler may not turn into one precomputed address per unrolled step
+// (they would cost the epilogue its registers)
+template <typename P> __device__ __forceinline__ void advance(P*& p, int64_t step) {
+  p += step;
+  asm volatile("" : "+l"(p));
+}
+template <typename T> __device__ __forceinline__ void store_pre1(void* pre, int64_t i, float f, bool f32) {
+  if (f32) static_cast<float*>(pre)[i] = f;
+  else static_cast<T*>(pre)[i] = from_acc<T>(f);
 }
 
 // ------------------------------------------------------------------ pair GEMM
@@ -110,9 +108,10 @@ constexpr int STAGES = 6;
 constexpr int TILE_BYTES = 128 * BK * 2;     // 16 KB, either major
 constexpr int HALF_TILE = TILE_BYTES / 2;    // MN-major: 64 MN elements x 64 K rows
 constexpr int STAGE_BYTES = 2 * TILE_BYTES;  // A + B of one CTA
-constexpr int NT = 256;
-constexpr int OFF_STAGING = STAGES * STAGE_BYTES;  // 4 epilogue warps x 32 rows x 32 float32
-constexpr int STAGING_BYTES = 4 * 32 * 32 * 4;
+constexpr int EPI_WARPS = 8;  // two per TMEM lane quadrant, each half of the columns
+constexpr int NT = 128 + 32 * EPI_WARPS;
+constexpr int OFF_STAGING = STAGES * STAGE_BYTES;  // per epilogue warp 32 rows x 32 float32
+constexpr int STAGING_BYTES = EPI_WARPS * 32 * 32 * 4;
 constexpr int OFF_BAR = OFF_STAGING + STAGING_BYTES;
 enum { B_FULL = 0, B_EMPTY = STAGES, B_ACCF = 2 * STAGES, B_ACCE = 2 * STAGES + 2, B_FINAL = 2 * STAGES + 4,
        NBAR = 2 * STAGES + 5 };
@@ -129,7 +128,8 @@ struct PairParams {
   int group;       // row blocks whose columns are walked together (operand reuse in L2)
   int n_units;
   int act;
-  int vec;         // every row of out / res / pre may be accessed four elements at a time
+  int vec;         // N is a multiple of 4 and every row of out / res / pre may be accessed four at a time
+  int pre_f32;     // pre is float32 (else of the activations' type)
   void* out0;
   void* out1;
   const void* bias;
@@ -171,11 +171,16 @@ __device__ __forceinline__ void load_tile_pair(uint8_t* dst, const CUtensorMap* 
   }
 }
 
-template <typename T, bool A_MN, bool B_MN, bool GATED>
+// what the epilogue does with an accumulator: store it, the plain product's whole epilogue, or the
+// gate's product
+enum { EPI_STORE = 0, EPI_LINEAR = 1, EPI_GATED = 2 };
+
+template <typename T, bool A_MN, bool B_MN, int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1)
 pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constant__ CUtensorMap tm_a1,
                  const __grid_constant__ CUtensorMap tm_b0, const __grid_constant__ CUtensorMap tm_b1,
                  const PairParams p) {
+  constexpr bool GATED = EPI == EPI_GATED;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + OFF_BAR);
@@ -186,7 +191,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
   const int pair = (int)(blockIdx.x >> 1), n_pairs = (int)(gridDim.x >> 1);
 
   if (tid == 0) {
-    for (int i = 0; i < NBAR; ++i) mbar_init(&bar[i], i == B_ACCE || i == B_ACCE + 1 ? 8 : 1);  // 4 warps x 2 CTAs
+    for (int i = 0; i < NBAR; ++i) mbar_init(&bar[i], i == B_ACCE || i == B_ACCE + 1 ? 2 * EPI_WARPS : 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -276,24 +281,47 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
     // ---------------------------------------------------------------- epilogue
     // A warp takes its 32 accumulator rows 32 columns at a time: one row per lane out of TMEM,
     // through shared memory (16-byte chunks swizzled by the row, no bank conflicts), so that
-    // eight lanes then hold one row's 32 columns and global accesses are 64-byte runs.
-    const int q = warp - 4;  // TMEM lane quadrant
+    // eight lanes then hold one row's 32 columns and global accesses are 64-byte runs; rows whose
+    // pitch or base does not allow that go one element per lane.  The residual of a chunk is read
+    // before its accumulators are waited for.
+    const int w = warp - 4, q = w & 3, half = w >> 2;  // TMEM lane quadrant, column half
+    constexpr int COLS = (GATED ? BN / 2 : BN) / 2;   // result columns of this warp
     const uint32_t acce = mapa_shared(&bar[B_ACCE], 0);
-    uint8_t* stage = smem + OFF_STAGING + q * (32 * 32 * 4);
+    uint8_t* stage = smem + OFF_STAGING + w * (32 * 32 * 4);
     const int rr = lane >> 3, cc = lane & 7;
-    const bool vec = p.vec != 0;
-    auto through_smem = [&](const uint32_t (&v)[32], float4 (&f)[8]) {
+    const bool vec = p.vec != 0, pre_f32 = p.pre_f32 != 0;
+    const T* res = EPI == EPI_LINEAR ? static_cast<const T*>(p.res) : nullptr;
+    const T* bias = EPI == EPI_LINEAR ? static_cast<const T*>(p.bias) : nullptr;
+    void* const pre = EPI == EPI_STORE ? nullptr : p.pre;
+    const int act = EPI == EPI_STORE ? KVS_ACT_NONE : p.act;
+    // addresses as 32-bit offsets formed at their use: row r, 16-byte chunk c lies at
+    // 128 r + 16 (c ^ (r & 7))
+    const uint32_t stage_at = smem_addr(stage);
+    const uint32_t put_at = stage_at + lane * 128 + ((lane & 7) << 4);
+    const uint32_t four_at = stage_at + rr * 128 + ((cc ^ rr) << 4);
+    auto to_smem = [&](const uint32_t (&v)[32]) {
       __syncwarp();
 #pragma unroll
       for (int c = 0; c < 8; ++c)
-        *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-            make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(put_at ^ (c << 4)), "r"(v[4 * c]),
+                     "r"(v[4 * c + 1]), "r"(v[4 * c + 2]), "r"(v[4 * c + 3])
+                     : "memory");
       __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = i * 4 + rr;
-        f[i] = *reinterpret_cast<const float4*>(stage + r * 128 + ((cc ^ (r & 7)) << 4));
-      }
+    };
+    // row 4 i + rr, columns 4 cc .. 4 cc + 3 (r & 7 = rr + 4 (i & 1): the chunk's bit 2 flips)
+    auto four = [&](int i) {
+      float4 f;
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];\n"
+                   : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
+                   : "r"((four_at ^ ((i & 1) << 6)) + i * 512));
+      return f;
+    };
+    auto single = [&](int r) {  // row r, column `lane`
+      float f;
+      asm volatile("ld.shared.f32 %0, [%1];\n"
+                   : "=f"(f)
+                   : "r"(stage_at + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4));
+      return f;
     };
     bool dead = false;
     int ui = 0;
@@ -301,66 +329,151 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
       const int ab = ui & 1;
       int part, mb, nb;
       unit_of(p, u, part, mb, nb);
-      const int row0 = mb * 2 * BM + (int)rank * BM + q * 32;
-      const int n0 = nb * (GATED ? BN / 2 : BN);
+      const int64_t row0 = (int64_t)mb * 2 * BM + (int)rank * BM + q * 32;
+      const int n0 = nb * (GATED ? BN / 2 : BN) + half * COLS;
+      const int rows = (int)min((int64_t)32, p.M - row0);  // existing rows of this warp
+      T* out = static_cast<T*>(part ? p.out1 : p.out0);
+      uint2 rv[8];  // the residual of the chunk at hand, four elements each
+      if (res && vec) {
+        const T* first = res + (row0 + rr) * p.ld_res + n0 + cc * 4;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (i * 4 + rr < rows && n0 + cc * 4 < p.N) rv[i] = *reinterpret_cast<const uint2*>(first);
+          advance(first, 4 * p.ld_res);
+        }
+      }
       if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(&bar[B_ACCF + ab], (ui >> 1) & 1, abort_flag));
       if (dead && lane == 0) *abort_flag = 1;
       tc_fence_after();
-      const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + ab * BN;
-      T* out = static_cast<T*>(part ? p.out1 : p.out0);
-      const T* res = static_cast<const T*>(p.res);
-      T* pre = static_cast<T*>(p.pre);
+      const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + ab * BN + half * COLS;
 #pragma unroll 1
-      for (int c = 0; c < (GATED ? BN / 2 : BN) / 32; ++c) {
-        const int col = n0 + c * 32 + cc * 4;
-        const int nv = p.N - col;  // existing columns from `col` on
+      for (int c = 0; c < COLS / 32; ++c) {
         if (n0 + c * 32 >= p.N) break;
+        const int col = n0 + c * 32 + (vec ? cc * 4 : lane);
+        const bool in = col < p.N;  // (vec: N is a multiple of 4)
         uint32_t v[32];
-        float4 f[8];
-        if (dead) {
+        if (!dead) {
+          tmem_ld32(taddr + c * 32, v);
+          if constexpr (!GATED) tmem_wait_ld();
+        } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = 0x7fc00000u;
-        } else {
-          tmem_ld32(taddr + c * 32, v);
-          tmem_wait_ld();
         }
-        through_smem(v, f);
         if constexpr (GATED) {
+          // g and u of one output lie in the same lane: the product is formed before the exchange
+          uint32_t u32[32];
           if (!dead) {
-            tmem_ld32(taddr + BN / 2 + c * 32, v);
+            tmem_ld32(taddr + BN / 2 + c * 32, u32);
             tmem_wait_ld();
-          }
-          float4 w[8];
-          through_smem(v, w);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int64_t row = row0 + i * 4 + rr;
-            if (row >= p.M || nv <= 0) continue;
-            if (pre) {
-              store4(pre + row * p.ld_pre + col, f[i], nv, vec);
-              store4(pre + row * p.ld_pre + p.N + col, w[i], nv, vec);
-            }
-            const float4 h = make_float4(act_f(f[i].x, p.act) * w[i].x, act_f(f[i].y, p.act) * w[i].y,
-                                         act_f(f[i].z, p.act) * w[i].z, act_f(f[i].w, p.act) * w[i].w);
-            store4(out + row * p.ld_out + col, h, nv, vec);
+            for (int j = 0; j < 32; ++j) u32[j] = 0x7fc00000u;
           }
-        } else {
-          float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (p.bias && nv > 0) b = load4(static_cast<const T*>(p.bias) + col, nv, vec);
+          // the chunk in shared memory to 32 rows of `to`
+          auto rows_to = [&](auto* to, int64_t ld) {
+            if (vec) {
+              to += (row0 + rr) * ld + col;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int64_t row = row0 + i * 4 + rr;
-            if (row >= p.M || nv <= 0) continue;
-            const float4 z = make_float4(f[i].x + b.x, f[i].y + b.y, f[i].z + b.z, f[i].w + b.w);
-            if (pre) store4(pre + row * p.ld_pre + col, z, nv, vec);
-            float4 y = make_float4(act_f(z.x, p.act), act_f(z.y, p.act), act_f(z.z, p.act), act_f(z.w, p.act));
-            if (res) {
-              const float4 r = load4(res + row * p.ld_res + col, nv, vec);
-              y = make_float4(y.x + r.x, y.y + r.y, y.z + r.z, y.w + r.w);
+              for (int i = 0; i < 8; ++i) {
+                if (i * 4 + rr < rows && in) store4(to, four(i));
+                advance(to, 4 * ld);
+              }
+            } else {
+              to += row0 * ld + col;
+#pragma unroll 4
+              for (int r = 0; r < rows; ++r) {
+                if (in) *to = from_acc<std::remove_reference_t<decltype(*to)>>(single(r));
+                advance(to, ld);
+              }
             }
-            store4(out + row * p.ld_out + col, y, nv, vec);
+          };
+          auto keep = [&](const uint32_t(&s)[32], int64_t off) {
+            to_smem(s);
+            if (pre_f32) rows_to(static_cast<float*>(pre) + off, p.ld_pre);
+            else rows_to(static_cast<T*>(pre) + off, p.ld_pre);
+          };
+          if (pre) {
+            keep(v, 0);
+            keep(u32, p.N);
           }
+          auto gate = [&](auto code) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              v[j] = __float_as_uint(act_f(__uint_as_float(v[j]), decltype(code)::value) * __uint_as_float(u32[j]));
+          };
+          if (act == KVS_ACT_SILU) gate(std::integral_constant<int, KVS_ACT_SILU>());
+          else if (act == KVS_ACT_GELU) gate(std::integral_constant<int, KVS_ACT_GELU>());
+          else if (act == KVS_ACT_RELU) gate(std::integral_constant<int, KVS_ACT_RELU>());
+          else gate(std::integral_constant<int, KVS_ACT_NONE>());
+          to_smem(v);
+          rows_to(out, p.ld_out);
+          continue;
         }
+        to_smem(v);
+        auto finish = [&](auto code) {
+          constexpr int ACT = decltype(code)::value;
+          if (vec) {
+            float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (bias && in) b = load4(bias + col);
+            T* o = out + (row0 + rr) * p.ld_out + col;
+            const T* next = res + (row0 + rr) * p.ld_res + col + 32;
+            const bool more = (c + 1) * 32 < COLS && col + 32 < p.N;
+            int64_t pi = (row0 + rr) * p.ld_pre + col;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const bool on = i * 4 + rr < rows && in;
+              const float4 f = four(i);
+              const float4 z = make_float4(f.x + b.x, f.y + b.y, f.z + b.z, f.w + b.w);
+              if (pre) {
+                if (on) store_pre<T>(pre, pi, z, pre_f32);
+                pi += 4 * p.ld_pre;
+                asm volatile("" : "+l"(pi));
+              }
+              float4 y = make_float4(act_f(z.x, ACT), act_f(z.y, ACT), act_f(z.z, ACT), act_f(z.w, ACT));
+              if (res) {  // the next chunk's load goes out as soon as this one's value is taken
+                Vec4<T> r4;
+                *reinterpret_cast<uint2*>(&r4) = rv[i];
+                y.x += to_acc<T>(r4.v[0]);
+                y.y += to_acc<T>(r4.v[1]);
+                y.z += to_acc<T>(r4.v[2]);
+                y.w += to_acc<T>(r4.v[3]);
+                if (more && i * 4 + rr < rows) rv[i] = *reinterpret_cast<const uint2*>(next);
+                advance(next, 4 * p.ld_res);
+              }
+              if (on) store4(o, y);
+              advance(o, 4 * p.ld_out);
+            }
+          } else {
+            const float b = bias && in ? to_acc<T>(bias[col]) : 0.f;
+            T* o = out + row0 * p.ld_out + col;
+            const T* rp = res + row0 * p.ld_res + col;
+            int64_t pi = row0 * p.ld_pre + col;
+#pragma unroll 1
+            for (int r0 = 0; r0 < rows; r0 += 8) {
+              float y[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                y[i] = res && r0 + i < rows && in ? to_acc<T>(*rp) : 0.f;
+                if (res) advance(rp, p.ld_res);
+              }
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int r = r0 + i;
+                if (r < rows && in) {
+                  const float z = single(r) + b;
+                  if (pre) store_pre1<T>(pre, pi + i * p.ld_pre, z, pre_f32);
+                  *o = from_acc<T>(act_f(z, ACT) + y[i]);
+                }
+                advance(o, p.ld_out);
+              }
+              pi += 8 * p.ld_pre;
+            }
+          }
+        };
+        if (EPI == EPI_STORE || act == KVS_ACT_NONE) finish(std::integral_constant<int, KVS_ACT_NONE>());
+        else if (act == KVS_ACT_SILU) finish(std::integral_constant<int, KVS_ACT_SILU>());
+        else if (act == KVS_ACT_GELU) finish(std::integral_constant<int, KVS_ACT_GELU>());
+        else finish(std::integral_constant<int, KVS_ACT_RELU>());
       }
       // this thread's TMEM reads are done: release the accumulator to the MMA warp
       tc_fence_before();
@@ -377,12 +490,21 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
 }
 
 // ------------------------------------------------------------------ gradients of the epilogue
+// eight consecutive elements, zeros from the n-th on
+template <typename T> __device__ __forceinline__ Vec8<T> load8(const T* p, int n, bool vec) {
+  if (vec) return *reinterpret_cast<const Vec8<T>*>(p);
+  Vec8<T> r;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) r.v[k] = k < n ? p[k] : from_acc<T>(0.f);
+  return r;
+}
+
 // dz = gy act'(pre) (or gy itself) into a row pitch the tensor maps take, and its column sums
 // over a chunk of rows (the bias gradient's partials, added up in chunk order: the bits do not
 // depend on scheduling).  64 x 4 threads: eight columns each, rows in steps of four.
-template <typename T>
+template <typename T, typename Z>
 __global__ void __launch_bounds__(256)
-dz_kernel(const T* __restrict__ gy, int64_t ld_gy, const T* __restrict__ pre, int64_t ld_pre, int act,
+dz_kernel(const T* __restrict__ gy, int64_t ld_gy, const Z* __restrict__ pre, int64_t ld_pre, int act,
           T* __restrict__ dz, int64_t ld_dz, float* __restrict__ part, int M, int N, int rows_per, int vec) {
   __shared__ float red[4][512];
   const int c0 = (blockIdx.x * 64 + threadIdx.x) * 8;
@@ -392,24 +514,17 @@ dz_kernel(const T* __restrict__ gy, int64_t ld_gy, const T* __restrict__ pre, in
   if (nv > 0) {
     for (int r = blockIdx.y * rows_per + threadIdx.y; r < r_end; r += 4) {
       const T* g = gy + (int64_t)r * ld_gy + c0;
-      const T* z = pre ? pre + (int64_t)r * ld_pre + c0 : nullptr;
-      Vec8<T> gv, zv, o;
-      if (vec) {
-        gv = *reinterpret_cast<const Vec8<T>*>(g);
-        if (z) zv = *reinterpret_cast<const Vec8<T>*>(z);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          gv.v[k] = k < nv ? g[k] : from_acc<T>(0.f);
-          if (z) zv.v[k] = k < nv ? z[k] : from_acc<T>(0.f);
-        }
-      }
+      const Z* z = pre ? pre + (int64_t)r * ld_pre + c0 : nullptr;
+      Vec8<T> o;
+      const Vec8<T> gv = load8(g, nv, vec);
+      Vec8<Z> zv;
+      if (z) zv = load8(z, nv, vec);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         float d = to_acc<T>(gv.v[k]);
         if (z) {
           float a, da;
-          act_grad_f(to_acc<T>(zv.v[k]), act, a, da);
+          act_grad_f(to_acc<Z>(zv.v[k]), act, a, da);
           d *= da;
         }
         sum[k] += d;
@@ -439,38 +554,25 @@ __global__ void bias_grad_kernel(const float* __restrict__ part, T* __restrict__
 
 // dg = gh u act'(g) and du = gh act(g), eight columns per thread; dgu rows hold dg at 0 and du
 // at `half` (N rounded up to 8), zeros between
-template <typename T>
+template <typename T, typename Z>
 __global__ void __launch_bounds__(256)
-gated_dz_kernel(const T* __restrict__ gh, int64_t ld_gh, const T* __restrict__ pre, int64_t ld_pre, int act,
+gated_dz_kernel(const T* __restrict__ gh, int64_t ld_gh, const Z* __restrict__ pre, int64_t ld_pre, int act,
                 T* __restrict__ dgu, int64_t ld_dgu, int half, int64_t M, int N, int vec) {
   const int nvec = half / 8;
   for (int64_t idx = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; idx < M * nvec;
        idx += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = idx / nvec;
     const int c0 = (int)(idx - r * nvec) * 8, nv = N - c0;
-    const T* g = pre + r * ld_pre + c0;
-    const T* u = g + N;
-    const T* h = gh + r * ld_gh + c0;
-    Vec8<T> gv, uv, hv, og, ou;
-    if (vec) {
-      gv = *reinterpret_cast<const Vec8<T>*>(g);
-      uv = *reinterpret_cast<const Vec8<T>*>(u);
-      hv = *reinterpret_cast<const Vec8<T>*>(h);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const T zero = from_acc<T>(0.f);
-        gv.v[k] = k < nv ? g[k] : zero;
-        uv.v[k] = k < nv ? u[k] : zero;
-        hv.v[k] = k < nv ? h[k] : zero;
-      }
-    }
+    const Z* g = pre + r * ld_pre + c0;
+    const Vec8<Z> gv = load8(g, nv, vec), uv = load8(g + N, nv, vec);
+    const Vec8<T> hv = load8(gh + r * ld_gh + c0, nv, vec);
+    Vec8<T> og, ou;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       float a, da;
-      act_grad_f(to_acc<T>(gv.v[k]), act, a, da);
+      act_grad_f(to_acc<Z>(gv.v[k]), act, a, da);
       const float hf = to_acc<T>(hv.v[k]);
-      og.v[k] = from_acc<T>(hf * to_acc<T>(uv.v[k]) * da);
+      og.v[k] = from_acc<T>(hf * to_acc<Z>(uv.v[k]) * da);
       ou.v[k] = from_acc<T>(hf * a);
     }
     *reinterpret_cast<Vec8<T>*>(dgu + r * ld_dgu + c0) = og;
@@ -558,10 +660,11 @@ struct Product {
   PairParams p = {};
 };
 
-template <typename T, bool A_MN, bool B_MN, bool GATED>
+template <typename T, bool A_MN, bool B_MN, int EPI>
 int launch_pair(const Product& g, int32_t dtype, cudaStream_t st) {
+  constexpr bool GATED = EPI == EPI_GATED;
   static KernelState state;
-  const auto kernel = pair_gemm_kernel<T, A_MN, B_MN, GATED>;
+  const auto kernel = pair_gemm_kernel<T, A_MN, B_MN, EPI>;
   const int most = max_pairs(kernel, state);
   if (most <= 0) return KVS_E_UNSUPPORTED;
   CUtensorMap m[4];
@@ -598,6 +701,7 @@ int check_common(const kvs_linear_args* a) {
       !al(a->x, 16) || !al(a->weight, 16) || !al(a->weight_up, 16))
     return KVS_E_UNSUPPORTED;
   if (a->weight_up && (a->bias || a->residual)) return KVS_E_ARG;
+  if (a->pre && a->pre_dtype != KVS_F32 && a->pre_dtype != a->dtype) return KVS_E_UNSUPPORTED;
   return KVS_OK;
 }
 
@@ -616,13 +720,14 @@ template <typename T> int forward(const kvs_linear_args* a, cudaStream_t st) {
   p.bias = a->bias;
   p.res = a->residual;
   p.pre = a->pre;
+  p.pre_f32 = a->pre_dtype == KVS_F32;
   p.ld_out = a->ld_out;
   p.ld_res = a->ld_res;
   p.ld_pre = a->ld_pre;
-  p.vec = a->ld_out % 4 == 0 && al(a->out, 8) && al(a->bias, 8) && (!a->residual || (a->ld_res % 4 == 0 && al(a->residual, 8))) &&
-          (!a->pre || (a->ld_pre % 4 == 0 && al(a->pre, 8) && (!a->weight_up || a->n % 4 == 0)));
-  return a->weight_up ? launch_pair<T, false, false, true>(g, a->dtype, st)
-                      : launch_pair<T, false, false, false>(g, a->dtype, st);
+  p.vec = a->n % 4 == 0 && a->ld_out % 4 == 0 && al(a->out, 8) && al(a->bias, 8) && (!a->residual || (a->ld_res % 4 == 0 && al(a->residual, 8))) &&
+          (!a->pre || (a->ld_pre % 4 == 0 && al(a->pre, a->pre_dtype == KVS_F32 ? 16 : 8)));
+  return a->weight_up ? launch_pair<T, false, false, EPI_GATED>(g, a->dtype, st)
+                      : launch_pair<T, false, false, EPI_LINEAR>(g, a->dtype, st);
 }
 
 // rows per chunk of the bias-gradient partials: at most 256 chunks, enough of them that the
@@ -639,20 +744,20 @@ bool needs_dz(const kvs_linear_args* a, const kvs_linear_grads* g) {
   return a->activation != KVS_ACT_NONE || !al(g->gy, 16) || (a->rows > 1 && g->ld_gy % 8);
 }
 
-template <typename T> int backward(const kvs_linear_args* a, const kvs_linear_grads* g, cudaStream_t st) {
+template <typename T, typename Z> int backward(const kvs_linear_args* a, const kvs_linear_grads* g, cudaStream_t st) {
   const bool gated = a->weight_up != nullptr;
   const int M = a->rows, N = a->n, K = a->k;
   const int64_t pitch = up8(N);
   uint8_t* sp = static_cast<uint8_t*>(g->scratch);
   const T* gy = static_cast<const T*>(g->gy);
-  const T* pre = static_cast<const T*>(a->pre);
+  const Z* pre = static_cast<const Z*>(a->pre);
   Operand dz[2];
   int rc;
   if (gated) {
     const bool vec = N % 8 == 0 && al(gy, 16) && al(pre, 16) && g->ld_gy % 8 == 0 && a->ld_pre % 8 == 0;
     T* dgu = reinterpret_cast<T*>(sp);
     const int64_t work = (int64_t)M * (pitch / 8);
-    gated_dz_kernel<T><<<(unsigned)std::min<int64_t>((work + 255) / 256, 148 * 16), 256, 0, st>>>(
+    gated_dz_kernel<T, Z><<<(unsigned)std::min<int64_t>((work + 255) / 256, 148 * 16), 256, 0, st>>>(
         gy, g->ld_gy, pre, a->ld_pre, a->activation, dgu, 2 * pitch, (int)pitch, M, N, vec);
     if ((rc = launch_rc())) return rc;
     dz[0] = {dgu, M, N, 2 * pitch};
@@ -670,7 +775,7 @@ template <typename T> int backward(const kvs_linear_args* a, const kvs_linear_gr
       float* part = g->db ? reinterpret_cast<float*>(sp) : nullptr;
       const bool act = a->activation != KVS_ACT_NONE;
       const bool vec = N % 8 == 0 && al(gy, 16) && g->ld_gy % 8 == 0 && (!act || (al(pre, 16) && a->ld_pre % 8 == 0));
-      dz_kernel<T><<<dim3((N + 511) / 512, chunks), dim3(64, 4), 0, st>>>(
+      dz_kernel<T, Z><<<dim3((N + 511) / 512, chunks), dim3(64, 4), 0, st>>>(
           gy, g->ld_gy, act ? pre : nullptr, a->ld_pre, a->activation, own_dz, pitch, part, M, N, per, vec);
       if ((rc = launch_rc())) return rc;
       if (part) {
@@ -693,7 +798,7 @@ template <typename T> int backward(const kvs_linear_args* a, const kvs_linear_gr
     x.p.out0 = g->dx;
     x.p.ld_out = g->ld_dx;
     x.p.vec = g->ld_dx % 4 == 0 && al(g->dx, 8);
-    if ((rc = launch_pair<T, false, true, false>(x, a->dtype, st))) return rc;
+    if ((rc = launch_pair<T, false, true, EPI_STORE>(x, a->dtype, st))) return rc;
   }
   if (g->dw) {  // [N][K] = dz^T [N][M] x [M][K], summed over the rows (two results when gated)
     Product w;
@@ -709,7 +814,7 @@ template <typename T> int backward(const kvs_linear_args* a, const kvs_linear_gr
     w.p.out1 = g->dw_up;
     w.p.ld_out = g->ld_dw;
     w.p.vec = g->ld_dw % 4 == 0 && al(g->dw, 8) && al(g->dw_up, 8);
-    if ((rc = launch_pair<T, true, true, false>(w, a->dtype, st))) return rc;
+    if ((rc = launch_pair<T, true, true, EPI_STORE>(w, a->dtype, st))) return rc;
   }
   return KVS_OK;
 }
@@ -757,5 +862,7 @@ KVS_API int kvs_linear_backward(const kvs_linear_args* a, const kvs_linear_grads
   if ((g->dx && !al(g->dx, 2)) || (g->dw && !al(g->dw, 2))) return KVS_E_ARG;
   const size_t need = kvs_linear_backward_scratch_bytes(a, g);
   if (need && (!g->scratch || g->scratch_bytes < need || !al(g->scratch, 256))) return KVS_E_SCRATCH;
-  return a->dtype == KVS_F16 ? backward<__half>(a, g, st) : backward<__nv_bfloat16>(a, g, st);
+  const bool f32 = a->pre_dtype == KVS_F32;
+  if (a->dtype == KVS_F16) return f32 ? backward<__half, float>(a, g, st) : backward<__half, __half>(a, g, st);
+  return f32 ? backward<__nv_bfloat16, float>(a, g, st) : backward<__nv_bfloat16, __nv_bfloat16>(a, g, st);
 }

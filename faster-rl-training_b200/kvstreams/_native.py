@@ -188,7 +188,7 @@ class KvsLinearArgs(C.Structure):
         ("k", C.c_int32),
         ("dtype", C.c_int32),
         ("activation", C.c_int32),
-        ("reserved", C.c_int32),
+        ("pre_dtype", C.c_int32),
     ]
 
 

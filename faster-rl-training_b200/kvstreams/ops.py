@@ -538,9 +538,19 @@ def _product_args(x, weight, weight_up, activation):
     return a, keep
 
 
-def pre_buffer(x: torch.Tensor, width: int) -> torch.Tensor:
-    """Buffer for the pre-activations of a product of ``x``: ``[..., width]`` of its type."""
-    return torch.empty(*x.shape[:-1], width, dtype=x.dtype, device=x.device)
+def pre_buffer(x: torch.Tensor, width: int, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """Buffer for the pre-activations of a product of ``x``: ``[..., width]``, float32 or, for half
+    the memory and one more rounding in the gradients, the type of ``x``."""
+    return torch.empty(*x.shape[:-1], width, dtype=dtype, device=x.device)
+
+
+def _set_pre(a, pre: torch.Tensor, x: torch.Tensor, shape, p2) -> torch.Tensor:
+    if pre.dtype not in (torch.float32, x.dtype) or pre.device != x.device or tuple(pre.shape) != tuple(shape):
+        raise ValueError(f"pre must be a float32 or {x.dtype} tensor of shape {tuple(shape)} on {x.device} "
+                         f"(got {pre.dtype} {tuple(pre.shape)} on {pre.device})")
+    rows = p2(pre)
+    a.pre, a.ld_pre, a.pre_dtype = rows.data_ptr(), _ld(rows), N.DTYPE_CODE[pre.dtype]
+    return rows
 
 
 def _product(x, weight, weight_up, activation, bias, residual, pre, out):
@@ -564,9 +574,7 @@ def _product(x, weight, weight_up, activation, bias, residual, pre, out):
         keep.append(r2)
     if pre is not None:
         width = n if weight_up is None else 2 * n
-        _same("pre", pre, x, (*lead, width))
-        p2 = _out_rows("pre", pre, width)
-        a.pre, a.ld_pre = p2.data_ptr(), _ld(p2)
+        _set_pre(a, pre, x, (*lead, width), lambda p: _out_rows("pre", p, width))
     with _on(x):
         N.check(N.lib().kvs_linear(C.byref(a), N.stream_ptr(x.device)), "kvs_linear")
     return out
@@ -601,10 +609,7 @@ def _product_backward(gy, x, weight, weight_up, pre, activation, bias_grad):
         if pre is None:
             raise ValueError("the backward of an activation needs the forward's pre buffer")
         width = n if weight_up is None else 2 * n
-        _same("pre", pre, x, (*lead, width))
-        p2 = _dense_rows(pre, width)
-        a.pre, a.ld_pre = p2.data_ptr(), _ld(p2)
-        keep.append(p2)
+        keep.append(_set_pre(a, pre, x, (*lead, width), lambda p: _dense_rows(p, width)))
     dx = torch.empty(*lead, k, dtype=x.dtype, device=x.device)
     dw = torch.empty(n, k, dtype=x.dtype, device=x.device)
     du = torch.empty_like(dw) if weight_up is not None else None

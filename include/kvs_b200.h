@@ -493,7 +493,8 @@ int kvs_silu_mul_backward(const void* gu, const void* grad, void* dgu, int64_t n
  *   weight_up given: out = act(x W^T) * (x W_up^T)            (no bias, no residual)
  * x [rows][k], W and W_up [n][k] (a Linear layer's weight), bias [n], residual and out [rows][n];
  * rows are ld_* elements apart.  pre (optional) receives the pre-activations for the backward:
- * [rows][n], or [rows][2 n] = gate | up (the layout kvs_silu_mul reads).  out may be the residual.
+ * [rows][n], or [rows][2 n] = gate | up, in pre_dtype (KVS_F32, or dtype: half the memory, one more
+ * rounding in the gradients).  out may be the residual.
  * Any rows (0: nothing happens) and n; k and the pitches of x and the weights multiples of 8, their
  * bases 16-byte aligned (KVS_E_UNSUPPORTED otherwise).  A bounded wait inside a kernel that runs
  * out gives NaN outputs. */
@@ -517,7 +518,7 @@ typedef struct kvs_linear_args {
   int32_t k;
   int32_t dtype;
   int32_t activation;
-  int32_t reserved;
+  int32_t pre_dtype;
 } kvs_linear_args;
 int kvs_linear(const kvs_linear_args* a, kvs_stream_t stream);
 

@@ -131,8 +131,10 @@ def test_in_place_and_strided_rows():
     wide = torch.full((7, 400), 7.0, device="cuda")
     wide[:, 3:336] = x
     view = wide[:, 3:336]
+    # where a row's 16-byte loads begin decides the order of its sum, so the strided rows' loss
+    # is held to the float64 bound, not to the packed rows' bits; the gradient is elementwise
+    _check(view, ids, t, grad, 1.0, torch.float32)
     loss, lse = ops.distill(x, ids, t)
-    assert torch.equal(ops.distill(view, ids, t)[0], loss)
     want = ops.distill_backward(x, ids, t, lse, grad)
     assert torch.equal(ops.distill_backward(view, ids, t, lse, grad), want)
     got = ops.distill_backward(view, ids, t, lse, grad, out=view)

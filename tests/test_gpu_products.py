@@ -7,9 +7,8 @@ k * 2^-24 * sum|x w| and in practice far less: ACC = 2^-18 * sum|x||w| bounds it
 rounding errors of either sign (64 ulps of the absolute sum), the activations add a few float32 ulps
 (covered by the same term) and the final rounding adds eps / 2 of the value.  A backward output is a
 sum of products of two rounded operands: dz carries half a step of its own (eps / 2) and, with an
-activation, the half step of the kept pre-activation times the activation's curvature, so each term
-is off by at most (eps / 2)(1 + C) relative to gy's scale; the bound is that share of the absolute
-sum.  The absolute sums are computed in float64 beside the result."""
+activation, the rounding of the kept pre-activation (2^-24, or half a step of the operands' type) times
+the activation's curvature; the bound is that share of the absolute sum.  The absolute sums are computed in float64 beside the result."""
 
 import pytest
 import torch
@@ -54,37 +53,39 @@ def test_linear_forward(rows, n, k, act, dtype):
     x, w, b, r = _rand(g, rows, k, dtype=dtype), _rand(g, n, k, scale=0.1, dtype=dtype), _rand(g, n, dtype=dtype), _rand(g, rows, n, dtype=dtype)
     z0 = x.double() @ w.double().t()
     mass = (x.double().abs() @ w.double().abs().t()) * ACC
-    for bias, res in ((None, None), (b, r)):
-        pre = ops.pre_buffer(x, n)
+    for bias, res, pdt in ((None, None, torch.float32), (b, r, torch.float32), (b, None, dtype)):
+        pre = ops.pre_buffer(x, n, pdt)
         y = ops.linear(x, w, bias=bias, residual=res, activation=act, pre=pre)
         z = z0 if bias is None else z0 + bias.double()
         want = ACT[act](z) if res is None else ACT[act](z) + res.double()
         extra = mass * 2 + (z.abs() + 1) * 2.0 ** -20
-        _near(pre, z, extra, dtype, "pre")
+        _near(pre, z, extra, pdt, "pre")
         _near(y, want, extra, dtype, "y")
         assert torch.equal(y, ops.linear(x, w, bias=bias, residual=res, activation=act))  # pre changes nothing
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("act", [None, "relu", "silu", "gelu"])
+@pytest.mark.parametrize("keep_half", [False, True])
 @pytest.mark.parametrize("rows,n,k", SIZES)
-def test_linear_backward(rows, n, k, act, dtype):
+def test_linear_backward(rows, n, k, keep_half, act, dtype):
     from kvstreams import ops
 
     g = torch.Generator(device="cuda").manual_seed(rows * 5 + n + k)
     x, w, b, gy = _rand(g, rows, k, dtype=dtype), _rand(g, n, k, scale=0.1, dtype=dtype), _rand(g, n, dtype=dtype), _rand(g, rows, n, dtype=dtype)
-    pre = ops.pre_buffer(x, n)
+    pre = ops.pre_buffer(x, n, dtype if keep_half else torch.float32)
     ops.linear(x, w, bias=b, activation=act, pre=pre)
     dx, dw, db = ops.linear_backward(gy, x, w, pre=pre, activation=act, bias_grad=True)
     xd, wd, bd = (t.double().requires_grad_() for t in (x, w, b))
     z = F.linear(xd, wd, bd)
     want = torch.autograd.grad(ACT[act](z), [xd, wd, bd], gy.double())
-    # the derivative is taken at the kept pre-activation, half a step from z
+    # the derivative is taken at the kept pre-activation, half a step of its type from z
     slope, curv = SLOPE[act]
-    h = _half(dtype)
-    off = gy.double().abs() * (curv * (z.detach().abs() * h + 2.0 ** -16) + slope * (h + 2.0 ** -20))
+    h, hp = _half(dtype), _half(pre.dtype)
+    mass = (x.double().abs() @ w.double().abs().t() + b.double().abs()) * ACC + 2.0 ** -20
+    off = gy.double().abs() * (curv * (z.detach().abs() * hp + mass) + slope * (h + 2.0 ** -20))
     if act == "relu":  # z of either sign within the float32 sum's error of 0 may take either derivative
-        off = off + gy.double().abs() * (z.detach().abs() < 2.0 ** -12)
+        off = off + gy.double().abs() * (z.detach().abs() < mass)
     big = gy.double().abs() * slope
     _near(dx, want[0], off @ w.double().abs() + big @ w.double().abs() * ACC, dtype, "dx")
     _near(dw, want[1], off.t() @ x.double().abs() + big.t() @ x.double().abs() * ACC, dtype, "dw")
@@ -95,14 +96,15 @@ def test_linear_backward(rows, n, k, act, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("act", ["silu", "gelu", "relu", None])
+@pytest.mark.parametrize("keep_half", [False, True])
 @pytest.mark.parametrize("rows,n,k", SIZES)
-def test_gated_linear(rows, n, k, act, dtype):
+def test_gated_linear(rows, n, k, keep_half, act, dtype):
     from kvstreams import ops
 
     g = torch.Generator(device="cuda").manual_seed(rows * 3 + n + k)
     x, gh = _rand(g, rows, k, dtype=dtype), _rand(g, rows, n, dtype=dtype)
     wg, wu = _rand(g, n, k, scale=0.05, dtype=dtype), _rand(g, n, k, scale=0.05, dtype=dtype)
-    pre = ops.pre_buffer(x, 2 * n)
+    pre = ops.pre_buffer(x, 2 * n, dtype if keep_half else torch.float32)
     h = ops.gated_linear(x, wg, wu, activation=act, pre=pre)
     dx, dwg, dwu = ops.gated_linear_backward(gh, x, wg, wu, pre, activation=act)
     xd, gd, ud = (t.double().requires_grad_() for t in (x, wg, wu))
@@ -113,15 +115,15 @@ def test_gated_linear(rows, n, k, act, dtype):
     ax, ag, au = x.double().abs(), wg.double().abs(), wu.double().abs()
     mg, mu = ax @ ag.t() * ACC + 2.0 ** -20, ax @ au.t() * ACC + 2.0 ** -20  # float32 errors of g, u
     slope, curv = SLOPE[act]
-    _near(pre[:, :n], zg, mg, dtype, "gate")
-    _near(pre[:, n:], zu, mu, dtype, "up")
+    _near(pre[:, :n], zg, mg, pre.dtype, "gate")
+    _near(pre[:, n:], zu, mu, pre.dtype, "up")
     _near(h, y, slope * mg * (zu.abs() + mu) + (zg.abs() * slope + mg) * mu + y.abs() * 2.0 ** -20, dtype, "h")
     assert torch.equal(h, ops.gated_linear(x, wg, wu, activation=act))
-    hs = _half(dtype)
-    eg, eu = zg.abs() * hs + mg, zu.abs() * hs + mu  # how far the kept g, u are off
+    hs, hp = _half(dtype), _half(pre.dtype)
+    eg, eu = zg.abs() * hp + mg, zu.abs() * hp + mu  # how far the kept g, u are off
     gm = gh.double().abs()
     # dg = gh u act'(g): off by gh (eu slope + |u| curv eg), rounded (hs); du = gh act(g) likewise
-    jump = (zg.abs() < 2.0 ** -12).double() if act == "relu" else 0.0
+    jump = (zg.abs() < mg).double() if act == "relu" else 0.0
     og = gm * (eu * slope + (zu.abs() + eu) * (curv * eg + jump + slope * (hs + 2.0 ** -20)))
     ou = gm * (slope * eg + (zg.abs() + eg) * slope * (hs + 2.0 ** -20))
     bg, bu = gm * (zu.abs() * slope + 1), gm * (zg.abs() * slope + 1)
