@@ -77,23 +77,38 @@ template <typename T> __device__ __forceinline__ float4 load4(const T* p) {
   const Vec4<T> q = *reinterpret_cast<const Vec4<T>*>(p);
   return make_float4(to_acc<T>(q.v[0]), to_acc<T>(q.v[1]), to_acc<T>(q.v[2]), to_acc<T>(q.v[3]));
 }
+// two floats rounded to nearest into one register
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
 template <typename T> __device__ __forceinline__ void store4(T* p, float4 f) {
-  Vec4<T> q;
-  q.v[0] = from_acc<T>(f.x);
-  q.v[1] = from_acc<T>(f.y);
-  q.v[2] = from_acc<T>(f.z);
-  q.v[3] = from_acc<T>(f.w);
-  *reinterpret_cast<Vec4<T>*>(p) = q;
+  if constexpr (std::is_same<T, float>::value) *reinterpret_cast<float4*>(p) = f;
+  else *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(f.x, f.y), pack2<T>(f.z, f.w));
 }
-template <typename T> __device__ __forceinline__ void store_pre(void* pre, int64_t i, float4 f, bool f32) {
-  if (f32) store4(static_cast<float*>(pre) + i, f);
-  else store4(static_cast<T*>(pre) + i, f);
+// the first n of four elements; one access when `vec` (n is 4 then)
+template <typename T> __device__ __forceinline__ float4 load_n(const T* p, int n, bool vec) {
+  if (vec) return load4(p);
+  float4 r = make_float4(to_acc<T>(p[0]), 0.f, 0.f, 0.f);
+  if (n > 1) r.y = to_acc<T>(p[1]);
+  if (n > 2) r.z = to_acc<T>(p[2]);
+  if (n > 3) r.w = to_acc<T>(p[3]);
+  return r;
 }
-// a running pointer the compiler may not turn into one precomputed address per unrolled step
-// (they would cost the epilogue its registers)
-template <typename P> __device__ __forceinline__ void advance(P*& p, int64_t step) {
-  p += step;
-  asm volatile("" : "+l"(p));
+template <typename T> __device__ __forceinline__ void store_n(T* p, float4 f, int n, bool vec) {
+  if (vec) {
+    store4(p, f);
+    return;
+  }
+  p[0] = from_acc<T>(f.x);
+  if (n > 1) p[1] = from_acc<T>(f.y);
+  if (n > 2) p[2] = from_acc<T>(f.z);
+  if (n > 3) p[3] = from_acc<T>(f.w);
 }
 template <typename T> __device__ __forceinline__ void store_pre1(void* pre, int64_t i, float f, bool f32) {
   if (f32) static_cast<float*>(pre)[i] = f;
@@ -102,19 +117,18 @@ template <typename T> __device__ __forceinline__ void store_pre1(void* pre, int6
 
 // ------------------------------------------------------------------ pair GEMM
 constexpr int BM = 128;  // result rows per CTA (256 per pair)
-constexpr int BN = 256;  // accumulator columns per unit (128 per CTA's share of B)
 constexpr int BK = 64;   // reduced elements per stage
-constexpr int STAGES = 6;
 constexpr int TILE_BYTES = 128 * BK * 2;     // 16 KB, either major
 constexpr int HALF_TILE = TILE_BYTES / 2;    // MN-major: 64 MN elements x 64 K rows
-constexpr int STAGE_BYTES = 2 * TILE_BYTES;  // A + B of one CTA
 constexpr int EPI_WARPS = 8;  // two per TMEM lane quadrant, each half of the columns
 constexpr int NT = 128 + 32 * EPI_WARPS;
-constexpr int OFF_STAGING = STAGES * STAGE_BYTES;  // per epilogue warp 32 rows x 32 float32
+constexpr int RING_BYTES = 6 * 2 * TILE_BYTES;  // 6 stages of a 256-column unit, 8 of a 128-column one
+constexpr int MAX_STAGES = 8;
+constexpr int OFF_STAGING = RING_BYTES;  // per epilogue warp 32 rows x 32 float32
 constexpr int STAGING_BYTES = EPI_WARPS * 32 * 32 * 4;
 constexpr int OFF_BAR = OFF_STAGING + STAGING_BYTES;
-enum { B_FULL = 0, B_EMPTY = STAGES, B_ACCF = 2 * STAGES, B_ACCE = 2 * STAGES + 2, B_FINAL = 2 * STAGES + 4,
-       NBAR = 2 * STAGES + 5 };
+enum { B_FULL = 0, B_EMPTY = MAX_STAGES, B_ACCF = 2 * MAX_STAGES, B_ACCE = 2 * MAX_STAGES + 2,
+       B_FINAL = 2 * MAX_STAGES + 4, NBAR = 2 * MAX_STAGES + 5 };
 constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
 constexpr int PAIR_SMEM = OFF_MISC + 16 + 1024;  // + alignment slack
 static_assert(PAIR_SMEM <= 232448, "pair GEMM shared memory");
@@ -128,7 +142,7 @@ struct PairParams {
   int group;       // row blocks whose columns are walked together (operand reuse in L2)
   int n_units;
   int act;
-  int vec;         // N is a multiple of 4 and every row of out / res / pre may be accessed four at a time
+  int vec;         // N is a multiple of 8 and out, res, pre and bias suit 16-byte accesses and TMA
   int pre_f32;     // pre is float32 (else of the activations' type)
   void* out0;
   void* out1;
@@ -160,12 +174,12 @@ template <bool MN> __device__ __forceinline__ uint64_t operand_desc(uint32_t sad
   return MN ? desc_mnmajor_sw128(saddr, HALF_TILE) : desc_kmajor_sw128(saddr);
 }
 
-// 128 rows (MN index `row`) x 64 reduced elements (block kb) of an operand into `dst`
-template <bool MN>
+// ROWS rows (MN index from `row` on) x 64 reduced elements (block kb) of an operand into `dst`
+template <bool MN, int ROWS>
 __device__ __forceinline__ void load_tile_pair(uint8_t* dst, const CUtensorMap* map, int kb, int row, uint32_t bar) {
   if (MN) {  // map: inner index MN, outer K
     tma_load_2d_pair(dst, map, row, kb * BK, bar);
-    tma_load_2d_pair(dst + HALF_TILE, map, row + 64, kb * BK, bar);
+    if (ROWS > 64) tma_load_2d_pair(dst + HALF_TILE, map, row + 64, kb * BK, bar);
   } else {
     tma_load_2d_pair(dst, map, kb * BK, row, bar);
   }
@@ -175,12 +189,17 @@ __device__ __forceinline__ void load_tile_pair(uint8_t* dst, const CUtensorMap* 
 // gate's product
 enum { EPI_STORE = 0, EPI_LINEAR = 1, EPI_GATED = 2 };
 
-template <typename T, bool A_MN, bool B_MN, int EPI>
+template <typename T, bool A_MN, bool B_MN, int EPI, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1)
 pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constant__ CUtensorMap tm_a1,
                  const __grid_constant__ CUtensorMap tm_b0, const __grid_constant__ CUtensorMap tm_b1,
-                 const PairParams p) {
+                 const __grid_constant__ CUtensorMap tm_o0, const __grid_constant__ CUtensorMap tm_o1,
+                 const __grid_constant__ CUtensorMap tm_pre, const PairParams p) {
   constexpr bool GATED = EPI == EPI_GATED;
+  constexpr int B_BYTES = BN / 2 * BK * 2;  // a CTA's share of B
+  constexpr int STAGE_BYTES = TILE_BYTES + B_BYTES;
+  constexpr int STAGES = RING_BYTES / STAGE_BYTES;
+  static_assert(STAGES <= MAX_STAGES, "ring");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + OFF_BAR);
@@ -217,7 +236,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
         const int col = GATED ? nb * (BN / 2) : nb * BN + (int)rank * (BN / 2);
         for (int k = 0; k < kb_all; ++k, ++it) {
           const int s = it % STAGES;
-          if (it >= STAGES && !mbar_wait(&bar[B_EMPTY + s], ((it / STAGES) - 1) & 1, abort_flag)) {
+          if (it >= STAGES && !mbar_wait_fast(&bar[B_EMPTY + s], ((it / STAGES) - 1) & 1, abort_flag)) {
             ok = false;
             break;
           }
@@ -226,8 +245,8 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
           uint8_t* st = smem + s * STAGE_BYTES;
           const bool second = k >= p.n_kb;  // of two K parts
           const int kb = second ? k - p.n_kb : k;
-          load_tile_pair<A_MN>(st, part || second ? &tm_a1 : &tm_a0, kb, row, full);
-          load_tile_pair<B_MN>(st + TILE_BYTES, second || (GATED && rank) ? &tm_b1 : &tm_b0, kb, col, full);
+          load_tile_pair<A_MN, BM>(st, part || second ? &tm_a1 : &tm_a0, kb, row, full);
+          load_tile_pair<B_MN, BN / 2>(st + TILE_BYTES, second || (GATED && rank) ? &tm_b1 : &tm_b0, kb, col, full);
         }
       }
       if (!ok) *abort_flag = 1;
@@ -279,48 +298,76 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- epilogue
-    // A warp takes its 32 accumulator rows 32 columns at a time: one row per lane out of TMEM,
-    // through shared memory (16-byte chunks swizzled by the row, no bank conflicts), so that
-    // eight lanes then hold one row's 32 columns and global accesses are 64-byte runs; rows whose
-    // pitch or base does not allow that go one element per lane.  The residual of a chunk is read
-    // before its accumulators are waited for.
+    // A warp takes its 32 accumulator rows 32 columns at a time, one row per lane: bias, activation,
+    // gate and residual (16-byte loads of the lane's own row, one chunk ahead) in registers, the
+    // rounded row to shared memory (16-byte pieces, TMA's swizzle: no bank conflicts), and a TMA
+    // store writes the 32 x 32 box while the next chunk is computed (two buffers a warp; the float32
+    // pre-activations take both).  Where pitches or bases do not suit that (`vec` is 0) the float32
+    // chunk goes through shared memory instead and a lane takes a column.
     const int w = warp - 4, q = w & 3, half = w >> 2;  // TMEM lane quadrant, column half
     constexpr int COLS = (GATED ? BN / 2 : BN) / 2;   // result columns of this warp
     const uint32_t acce = mapa_shared(&bar[B_ACCE], 0);
-    uint8_t* stage = smem + OFF_STAGING + w * (32 * 32 * 4);
-    const int rr = lane >> 3, cc = lane & 7;
+    const uint32_t stage = smem_addr(smem + OFF_STAGING + w * (32 * 32 * 4));
     const bool vec = p.vec != 0, pre_f32 = p.pre_f32 != 0;
     const T* res = EPI == EPI_LINEAR ? static_cast<const T*>(p.res) : nullptr;
     const T* bias = EPI == EPI_LINEAR ? static_cast<const T*>(p.bias) : nullptr;
     void* const pre = EPI == EPI_STORE ? nullptr : p.pre;
     const int act = EPI == EPI_STORE ? KVS_ACT_NONE : p.act;
-    // addresses as 32-bit offsets formed at their use: row r, 16-byte chunk c lies at
-    // 128 r + 16 (c ^ (r & 7))
-    const uint32_t stage_at = smem_addr(stage);
-    const uint32_t put_at = stage_at + lane * 128 + ((lane & 7) << 4);
-    const uint32_t four_at = stage_at + rr * 128 + ((cc ^ rr) << 4);
-    auto to_smem = [&](const uint32_t (&v)[32]) {
+    // this lane's row of a 64-byte-row box (16-byte piece c at c ^ ((row >> 1) & 3)) and of a
+    // 128-byte-row box (at c ^ (row & 7))
+    const uint32_t row64 = lane * 64 + (((lane >> 1) & 3) << 4), row128 = stage + lane * 128 + ((lane & 7) << 4);
+    uint32_t flip = 0;  // which of the two 2 KB buffers is next
+    // 32 rounded values of this lane's row to the next buffer, and the box to x, y
+    auto put_half = [&](const CUtensorMap* map, const uint32_t (&o)[16], int x, int y) {
+      if (lane == 0) bulk_wait_read<1>();
+      __syncwarp();
+      const uint32_t at = stage + flip + row64;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) st_shared_u4(at ^ (c << 4), o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d(map, stage + flip, x, y);
+        bulk_commit();
+      }
+      flip ^= 2048;
+    };
+    auto put_f32 = [&](const CUtensorMap* map, const uint32_t (&v)[32], int x, int y) {  // both buffers
+      if (lane == 0) bulk_wait_read<0>();
       __syncwarp();
 #pragma unroll
-      for (int c = 0; c < 8; ++c)
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(put_at ^ (c << 4)), "r"(v[4 * c]),
-                     "r"(v[4 * c + 1]), "r"(v[4 * c + 2]), "r"(v[4 * c + 3])
-                     : "memory");
+      for (int c = 0; c < 8; ++c) st_shared_u4(row128 ^ (c << 4), v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d(map, stage, x, y);
+        bulk_commit();
+        bulk_wait_read<0>();
+      }
       __syncwarp();
     };
-    // row 4 i + rr, columns 4 cc .. 4 cc + 3 (r & 7 = rr + 4 (i & 1): the chunk's bit 2 flips)
-    auto four = [&](int i) {
-      float4 f;
-      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];\n"
-                   : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
-                   : "r"((four_at ^ ((i & 1) << 6)) + i * 512));
-      return f;
+    auto keep_pre = [&](const CUtensorMap* map, const uint32_t (&v)[32], int x, int y) {
+      if (pre_f32) {
+        put_f32(map, v, x, y);
+      } else {
+        uint32_t o[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j] = pack2<T>(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+        put_half(map, o, x, y);
+      }
     };
-    auto single = [&](int r) {  // row r, column `lane`
+    // the scalar path's exchange: row r, column `lane` of a float32 chunk
+    auto exchange = [&](const uint32_t (&v)[32]) {
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < 8; ++c) st_shared_u4(row128 ^ (c << 4), v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+      __syncwarp();
+    };
+    auto single = [&](int r) {
       float f;
       asm volatile("ld.shared.f32 %0, [%1];\n"
                    : "=f"(f)
-                   : "r"(stage_at + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4));
+                   : "r"(stage + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4));
       return f;
     };
     bool dead = false;
@@ -329,157 +376,130 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
       const int ab = ui & 1;
       int part, mb, nb;
       unit_of(p, u, part, mb, nb);
-      const int64_t row0 = (int64_t)mb * 2 * BM + (int)rank * BM + q * 32;
+      const int row0 = mb * 2 * BM + (int)rank * BM + q * 32;
       const int n0 = nb * (GATED ? BN / 2 : BN) + half * COLS;
-      const int rows = (int)min((int64_t)32, p.M - row0);  // existing rows of this warp
-      T* out = static_cast<T*>(part ? p.out1 : p.out0);
-      uint2 rv[8];  // the residual of the chunk at hand, four elements each
-      if (res && vec) {
-        const T* first = res + (row0 + rr) * p.ld_res + n0 + cc * 4;
+      const int rows = min(32, p.M - row0);  // existing rows of this warp (may be none)
+      uint4 rv[4];  // the residual of the chunk at hand
+      const T* rp = res + (int64_t)(row0 + lane) * p.ld_res + n0;
+      auto load_res = [&](int c) {
+        if (lane >= rows) return;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (i * 4 + rr < rows && n0 + cc * 4 < p.N) rv[i] = *reinterpret_cast<const uint2*>(first);
-          advance(first, 4 * p.ld_res);
-        }
-      }
+        for (int k = 0; k < 4; ++k)
+          if (n0 + c * 32 + k * 8 < p.N) rv[k] = *reinterpret_cast<const uint4*>(rp + c * 32 + k * 8);
+      };
+      if (res && vec) load_res(0);
       if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(&bar[B_ACCF + ab], (ui >> 1) & 1, abort_flag));
       if (dead && lane == 0) *abort_flag = 1;
       tc_fence_after();
       const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + ab * BN + half * COLS;
 #pragma unroll 1
       for (int c = 0; c < COLS / 32; ++c) {
-        if (n0 + c * 32 >= p.N) break;
-        const int col = n0 + c * 32 + (vec ? cc * 4 : lane);
-        const bool in = col < p.N;  // (vec: N is a multiple of 4)
-        uint32_t v[32];
+        const int col = n0 + c * 32;
+        if (col >= p.N || rows <= 0) break;
+        uint32_t v[32], u32[GATED ? 32 : 1];
         if (!dead) {
           tmem_ld32(taddr + c * 32, v);
-          if constexpr (!GATED) tmem_wait_ld();
+          if constexpr (GATED) tmem_ld32(taddr + BN / 2 + c * 32, u32);
+          tmem_wait_ld();
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = 0x7fc00000u;
-        }
-        if constexpr (GATED) {
-          // g and u of one output lie in the same lane: the product is formed before the exchange
-          uint32_t u32[32];
-          if (!dead) {
-            tmem_ld32(taddr + BN / 2 + c * 32, u32);
-            tmem_wait_ld();
-          } else {
+          if constexpr (GATED)
 #pragma unroll
             for (int j = 0; j < 32; ++j) u32[j] = 0x7fc00000u;
-          }
-          // the chunk in shared memory to 32 rows of `to`
-          auto rows_to = [&](auto* to, int64_t ld) {
-            if (vec) {
-              to += (row0 + rr) * ld + col;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                if (i * 4 + rr < rows && in) store4(to, four(i));
-                advance(to, 4 * ld);
-              }
-            } else {
-              to += row0 * ld + col;
-#pragma unroll 4
-              for (int r = 0; r < rows; ++r) {
-                if (in) *to = from_acc<std::remove_reference_t<decltype(*to)>>(single(r));
-                advance(to, ld);
-              }
-            }
-          };
-          auto keep = [&](const uint32_t(&s)[32], int64_t off) {
-            to_smem(s);
-            if (pre_f32) rows_to(static_cast<float*>(pre) + off, p.ld_pre);
-            else rows_to(static_cast<T*>(pre) + off, p.ld_pre);
-          };
-          if (pre) {
-            keep(v, 0);
-            keep(u32, p.N);
-          }
-          auto gate = [&](auto code) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              v[j] = __float_as_uint(act_f(__uint_as_float(v[j]), decltype(code)::value) * __uint_as_float(u32[j]));
-          };
-          if (act == KVS_ACT_SILU) gate(std::integral_constant<int, KVS_ACT_SILU>());
-          else if (act == KVS_ACT_GELU) gate(std::integral_constant<int, KVS_ACT_GELU>());
-          else if (act == KVS_ACT_RELU) gate(std::integral_constant<int, KVS_ACT_RELU>());
-          else gate(std::integral_constant<int, KVS_ACT_NONE>());
-          to_smem(v);
-          rows_to(out, p.ld_out);
-          continue;
         }
-        to_smem(v);
-        auto finish = [&](auto code) {
-          constexpr int ACT = decltype(code)::value;
-          if (vec) {
-            float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (bias && in) b = load4(bias + col);
-            T* o = out + (row0 + rr) * p.ld_out + col;
-            const T* next = res + (row0 + rr) * p.ld_res + col + 32;
-            const bool more = (c + 1) * 32 < COLS && col + 32 < p.N;
-            int64_t pi = (row0 + rr) * p.ld_pre + col;
+        if (!vec) {
+          // ------------------------------------------------ a lane per column
+          const bool in = col + lane < p.N;
+          T* out = static_cast<T*>(part ? p.out1 : p.out0) + (int64_t)row0 * p.ld_out + col + lane;
+          int64_t pi = (int64_t)row0 * p.ld_pre + col + lane;
+          if constexpr (GATED) {
+            if (pre)
+              for (int g = 0; g < 2; ++g) {
+                if (g) exchange(u32);
+                else exchange(v);
+#pragma unroll 1
+                for (int r = 0; r < rows; ++r)
+                  if (in) store_pre1<T>(pre, pi + r * p.ld_pre + g * p.N, single(r), pre_f32);
+              }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const bool on = i * 4 + rr < rows && in;
-              const float4 f = four(i);
-              const float4 z = make_float4(f.x + b.x, f.y + b.y, f.z + b.z, f.w + b.w);
-              if (pre) {
-                if (on) store_pre<T>(pre, pi, z, pre_f32);
-                pi += 4 * p.ld_pre;
-                asm volatile("" : "+l"(pi));
-              }
-              float4 y = make_float4(act_f(z.x, ACT), act_f(z.y, ACT), act_f(z.z, ACT), act_f(z.w, ACT));
-              if (res) {  // the next chunk's load goes out as soon as this one's value is taken
-                Vec4<T> r4;
-                *reinterpret_cast<uint2*>(&r4) = rv[i];
-                y.x += to_acc<T>(r4.v[0]);
-                y.y += to_acc<T>(r4.v[1]);
-                y.z += to_acc<T>(r4.v[2]);
-                y.w += to_acc<T>(r4.v[3]);
-                if (more && i * 4 + rr < rows) rv[i] = *reinterpret_cast<const uint2*>(next);
-                advance(next, 4 * p.ld_res);
-              }
-              if (on) store4(o, y);
-              advance(o, 4 * p.ld_out);
-            }
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(act_f(__uint_as_float(v[j]), act) * __uint_as_float(u32[j]));
+            exchange(v);
+#pragma unroll 4
+            for (int r = 0; r < rows; ++r)
+              if (in) out[r * p.ld_out] = from_acc<T>(single(r));
           } else {
-            const float b = bias && in ? to_acc<T>(bias[col]) : 0.f;
-            T* o = out + row0 * p.ld_out + col;
-            const T* rp = res + row0 * p.ld_res + col;
-            int64_t pi = row0 * p.ld_pre + col;
+            exchange(v);
+            const float b = bias && in ? to_acc<T>(bias[col + lane]) : 0.f;
+            const T* from = res + (int64_t)row0 * p.ld_res + col + lane;
 #pragma unroll 1
             for (int r0 = 0; r0 < rows; r0 += 8) {
               float y[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                y[i] = res && r0 + i < rows && in ? to_acc<T>(*rp) : 0.f;
-                if (res) advance(rp, p.ld_res);
-              }
+              for (int i = 0; i < 8; ++i) y[i] = res && r0 + i < rows && in ? to_acc<T>(from[(r0 + i) * p.ld_res]) : 0.f;
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 const int r = r0 + i;
-                if (r < rows && in) {
-                  const float z = single(r) + b;
-                  if (pre) store_pre1<T>(pre, pi + i * p.ld_pre, z, pre_f32);
-                  *o = from_acc<T>(act_f(z, ACT) + y[i]);
-                }
-                advance(o, p.ld_out);
+                if (r >= rows || !in) continue;
+                const float z = single(r) + b;
+                if (pre) store_pre1<T>(pre, pi + r * p.ld_pre, z, pre_f32);
+                out[r * p.ld_out] = from_acc<T>(act_f(z, act) + y[i]);
               }
-              pi += 8 * p.ld_pre;
             }
           }
+          continue;
+        }
+        // -------------------------------------------------- a lane per row
+        if constexpr (GATED) {
+          if (pre) {
+            keep_pre(&tm_pre, v, col, row0);
+            keep_pre(&tm_o1, u32, col, row0);
+          }
+        } else if (bias) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (col + k * 8 < p.N) {
+              const Vec8<T> b = *reinterpret_cast<const Vec8<T>*>(bias + col + k * 8);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[k * 8 + j] = __float_as_uint(__uint_as_float(v[k * 8 + j]) + to_acc<T>(b.v[j]));
+            }
+        }
+        if constexpr (EPI == EPI_LINEAR)
+          if (pre) keep_pre(&tm_pre, v, col, row0);
+        auto apply = [&](auto code) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float y = act_f(__uint_as_float(v[j]), decltype(code)::value);
+            if constexpr (GATED) y *= __uint_as_float(u32[j]);
+            v[j] = __float_as_uint(y);
+          }
         };
-        if (EPI == EPI_STORE || act == KVS_ACT_NONE) finish(std::integral_constant<int, KVS_ACT_NONE>());
-        else if (act == KVS_ACT_SILU) finish(std::integral_constant<int, KVS_ACT_SILU>());
-        else if (act == KVS_ACT_GELU) finish(std::integral_constant<int, KVS_ACT_GELU>());
-        else finish(std::integral_constant<int, KVS_ACT_RELU>());
+        if (EPI == EPI_STORE || act == KVS_ACT_NONE) apply(std::integral_constant<int, KVS_ACT_NONE>());
+        else if (act == KVS_ACT_SILU) apply(std::integral_constant<int, KVS_ACT_SILU>());
+        else if (act == KVS_ACT_GELU) apply(std::integral_constant<int, KVS_ACT_GELU>());
+        else apply(std::integral_constant<int, KVS_ACT_RELU>());
+        if (res) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            Vec8<T> r8;
+            *reinterpret_cast<uint4*>(&r8) = rv[k];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[k * 8 + j] = __float_as_uint(__uint_as_float(v[k * 8 + j]) + to_acc<T>(r8.v[j]));
+          }
+          if ((c + 1) * 32 < COLS) load_res(c + 1);
+        }
+        uint32_t o[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j] = pack2<T>(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+        put_half(part ? &tm_o1 : &tm_o0, o, col, row0);
       }
       // this thread's TMEM reads are done: release the accumulator to the MMA warp
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(acce + ab * 8);
     }
+    if (lane == 0) bulk_wait_read<0>();  // the boxes have left shared memory before the CTA does
+    __syncwarp();
   }
   tc_fence_before();
   cluster_sync();  // both CTAs done with TMEM and with each other's barriers
@@ -487,6 +507,272 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
     tc_fence_after();
     tmem_dealloc_pair(tmem, 512);
   }
+}
+
+// ------------------------------------------------------------------ stream GEMM (few rows)
+// With few rows of x the product is bound by reading the weights once.  The operands change
+// places: 128 weight rows (or, in dx, 128 columns of W) are the M = 128 rows of the MMA and a tile
+// of 16..256 rows of x its N columns, so the tensor cores' work follows the rows that exist and
+// TMEM lane = result column.  A cluster of S CTAs takes one tile and splits the reduced index
+// between them, so that (result tiles x S) CTAs stream the weights at once, two per SM while a
+// CTA's ring fits half of its shared memory; each holds about 100 KB of copies in flight.  The S
+// partial sums meet in distributed shared memory: CTA r adds up, in rank order, the 128 / S result
+// columns that it then finishes (bias, activation, gate product, residual) and stores.  Nothing
+// passes through global memory, no counters, no second launch, and the order of the sum is fixed.
+// The gated form's 128 weight rows are 64 of Wg and the 64 of Wu that belong to them: g and u of an
+// output are 64 columns apart in the partial sums.
+//
+// 256 threads: warp 0 lane 0 = TMA producer, warp 1 = TMEM allocation and MMA issuer, warps 4..7
+// take the accumulators to shared memory; all of them finish and store.
+constexpr int SNT = 256;
+constexpr int SMAX_STAGES = 8;
+constexpr int SMAX_SPLIT = 8;
+constexpr int HALF_SM_SMEM = 113 * 1024;  // two CTAs per SM: 228 KB less 1 KB each that the system keeps
+constexpr int S_BARS = 2 * SMAX_STAGES + 3;
+constexpr int S_BAR_BYTES = S_BARS * 8 + 8;
+
+struct StreamParams {
+  int M, N;      // rows of x (or dz), result columns
+  int n_kb;      // K blocks of one operand pair
+  int k_parts;   // 2: the sum runs over (weights 0, x 0), then (weights 1, x 1)
+  int tn;        // rows of x per tile, a multiple of 16
+  int nt;        // tiles of 128 result columns (64 when gated)
+  int stages;    // ring depth
+  int split;     // CTAs per tile (cluster size, a power of two)
+  int lsplit;    // its logarithm
+  int act, vec, pre_f32;
+  void* out;
+  const void* bias;
+  const void* res;
+  void* pre;
+  int64_t ld_out, ld_res, ld_pre;
+};
+
+template <typename T, bool W_MN, bool GATED>
+__global__ void __launch_bounds__(SNT)
+stream_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant__ CUtensorMap tm_w1,
+                   const __grid_constant__ CUtensorMap tm_x0, const __grid_constant__ CUtensorMap tm_x1,
+                   const StreamParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int COLS = GATED ? 64 : 128;  // result columns of a tile
+  const int stage_bytes = TILE_BYTES + p.tn * BK * 2;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + p.stages * stage_bytes);
+  uint64_t *full = bar, *empty = bar + SMAX_STAGES, *done = bar + 2 * SMAX_STAGES, *last = done + 1,
+           *drained = done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int tmem_cols = p.tn <= 32 ? 32 : p.tn <= 64 ? 64 : p.tn <= 128 ? 128 : 256;
+  const int rank = (int)(blockIdx.x % p.split);  // cluster rank (the clusters are along x)
+  const int tile = (int)(blockIdx.x / p.split);
+  const int n0 = (tile % p.nt) * COLS, m0 = (tile / p.nt) * p.tn;
+
+  if (tid == 0) {
+    for (int i = 0; i < S_BARS; ++i) mbar_init(&bar[i], 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // this CTA's share of the K blocks
+  const int kb_all = p.n_kb * p.k_parts;
+  const int kb_beg = (int)((int64_t)kb_all * rank / p.split), kb_end = (int)((int64_t)kb_all * (rank + 1) / p.split);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      int it = 0;
+      for (int k = kb_beg; k < kb_end; ++k, ++it) {
+        const int s = it % p.stages;
+        if (it >= p.stages && !mbar_wait_fast(&empty[s], ((it / p.stages) - 1) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(&full[s], stage_bytes);
+        uint8_t* st = smem + s * stage_bytes;
+        const bool second = k >= p.n_kb;
+        const int kb = second ? k - p.n_kb : k;
+        const CUtensorMap* w = second ? &tm_w1 : &tm_w0;
+        if (GATED) {  // (boxes of 64 rows)
+          tma_load_2d(st, &tm_w0, kb * BK, n0, &full[s]);
+          tma_load_2d(st + HALF_TILE, &tm_w1, kb * BK, n0, &full[s]);
+        } else if (W_MN) {
+          tma_load_2d(st, w, n0, kb * BK, &full[s]);
+          tma_load_2d(st + HALF_TILE, w, n0 + 64, kb * BK, &full[s]);
+        } else {
+          tma_load_2d(st, w, kb * BK, n0, &full[s]);
+        }
+        tma_load_2d(st + TILE_BYTES, second ? &tm_x1 : &tm_x0, kb * BK, m0, &full[s]);
+      }
+      if (!ok) *abort_flag = 1;
+      // every copy has landed before the CTA may go on to leave; immediate unless aborting
+      for (int j = max(0, it - p.stages); j < it; ++j)
+        mbar_wait(&full[j % p.stages], (j / p.stages) & 1, nullptr, ok ? 400000 : 20000);
+      mbar_arrive(drained);
+    }
+  } else if (warp == 1) {
+    const uint32_t idesc = idesc_of<T>(128, p.tn, W_MN, 0);
+    constexpr uint32_t AS = W_MN ? 128 : 2;
+    const uint32_t base = smem_addr(smem);
+    bool ok = true;
+    int it = 0;
+    for (int k = kb_beg; k < kb_end; ++k, ++it) {
+      const int s = it % p.stages;
+      ok = __all_sync(0xffffffffu, mbar_wait_fast(&full[s], (it / p.stages) & 1, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t at = base + s * stage_bytes;
+      const uint64_t dw = operand_desc<W_MN>(at), dx = desc_kmajor_sw128(at + TILE_BYTES);
+      umma_bf16_warp_at<0, 0>(tmem, dw, dx, idesc, it > 0);
+      umma_bf16_warp_at<AS, 2>(tmem, dw, dx, idesc, 1);
+      umma_bf16_warp_at<2 * AS, 4>(tmem, dw, dx, idesc, 1);
+      umma_bf16_warp_at<3 * AS, 6>(tmem, dw, dx, idesc, 1);
+      umma_commit_warp(&empty[s]);
+    }
+    if (ok) umma_commit_warp(done);
+    else if (lane == 0) *abort_flag = 1;
+    // every MMA issued has completed before TMEM is released
+    umma_commit_warp(last);
+    mbar_wait(last, 0, nullptr);
+    __syncwarp();
+  } else if (warp >= 4) {
+    // partial sums to shared memory, [row of x][128 weight rows]: over the ring,
+    // which nothing uses any more once the last MMA has completed
+    const int q = warp & 3;  // TMEM lane quadrant
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(done, 0, abort_flag));
+    if (!ok) {  // the NaNs go where copies may still be landing: after those
+      if (lane == 0) *abort_flag = 1;
+      mbar_wait(drained, 0, nullptr);
+      __syncwarp();
+    }
+    tc_fence_after();
+    const uint32_t part = smem_addr(smem) + (q * 32 + lane) * 4;
+    const int live = min(p.tn, p.M - m0);
+#pragma unroll 1
+    for (int c = 0; c < live; c += 32) {  // two loads in flight (the second may be past the tile)
+      uint32_t v[16], w[16];
+      const bool two = c + 16 < live;
+      if (ok) {
+        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, v);
+        if (two) tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + c + 16, w);
+        tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = w[j] = 0x7fc00000u;
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) st_shared_f1(part + (c + j) * 512, __uint_as_float(v[j]));
+      if (two)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) st_shared_f1(part + (c + 16 + j) * 512, __uint_as_float(w[j]));
+    }
+    tc_fence_before();
+  }
+  if (p.split > 1) cluster_sync();
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, tmem_cols);
+  }
+  {
+    // this CTA's share of the tile: 128 / S (64 / S) result columns in groups of four, one group per
+    // thread, and rows of x in steps of (threads / groups)
+    const int lq = (GATED ? 4 : 5) - p.lsplit;  // log2 of the groups
+    const int c = (((rank << lq) + (tid & ((1 << lq) - 1)))) * 4, n = n0 + c;
+    const int step = SNT >> lq;
+    const int live = n < p.N ? min(p.tn, p.M - m0) : 0;
+    int m = tid >> lq;
+    const T* bias = static_cast<const T*>(p.bias);
+    const bool pre_f32 = p.pre_f32 != 0, vec = p.vec != 0;  // (vec: N is a multiple of 4)
+    const int have = min(4, p.N - n);
+    float4 b4 = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (bias && live > 0) b4 = load_n(bias + n, have, vec);
+    uint32_t at = smem_addr(smem) + (m * 128 + c) * 4;
+    T* out = static_cast<T*>(p.out) + (int64_t)(m0 + m) * p.ld_out + n;
+    const T* res = static_cast<const T*>(p.res) + (int64_t)(m0 + m) * p.ld_res + n;
+    int64_t pi = (int64_t)(m0 + m) * p.ld_pre + n;
+    // four partial columns of a row of x: every CTA's are asked for before any is added, in rank order
+    auto ask = [&](auto s, uint32_t from, float4 (&v)[decltype(s)::value]) {
+      constexpr int S = decltype(s)::value;
+      if constexpr (S == 1) {
+        v[0] = ld_shared_f4(from);
+      } else {
+#pragma unroll
+        for (int r = 0; r < S; ++r) v[r] = ld_cluster_f4(mapa_addr(from, r));
+      }
+    };
+    auto add_up = [&](const auto& v) {
+      float4 t = v[0];
+#pragma unroll
+      for (int r = 1; r < (int)(sizeof(v) / sizeof(float4)); ++r)
+        t = make_float4(t.x + v[r].x, t.y + v[r].y, t.z + v[r].z, t.w + v[r].w);
+      return t;
+    };
+    auto finish = [&](auto code, float4 z, float4 u) {
+      constexpr int ACT = decltype(code)::value;
+      z = make_float4(z.x + b4.x, z.y + b4.y, z.z + b4.z, z.w + b4.w);
+      if (p.pre) {
+        if (pre_f32) {
+          store_n(static_cast<float*>(p.pre) + pi, z, have, vec);
+          if constexpr (GATED) store_n(static_cast<float*>(p.pre) + pi + p.N, u, have, vec);
+        } else {
+          store_n(static_cast<T*>(p.pre) + pi, z, have, vec);
+          if constexpr (GATED) store_n(static_cast<T*>(p.pre) + pi + p.N, u, have, vec);
+        }
+        pi += step * p.ld_pre;
+      }
+      float4 y = make_float4(act_f(z.x, ACT), act_f(z.y, ACT), act_f(z.z, ACT), act_f(z.w, ACT));
+      if constexpr (GATED) y = make_float4(y.x * u.x, y.y * u.y, y.z * u.z, y.w * u.w);
+      if (p.res) {
+        const float4 r = load_n(res, have, vec);
+        y = make_float4(y.x + r.x, y.y + r.y, y.z + r.z, y.w + r.w);
+        res += step * p.ld_res;
+      }
+      store_n(out, y, have, vec);
+      out += step * p.ld_out;
+    };
+    const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+    // One loop per activation and split: with both chosen at run time inside it, a row of four
+    // columns cost 540 issue cycles instead of about 60, more than the product itself at 64 rows.
+    auto rows = [&](auto code, auto s) {
+      constexpr int S = decltype(s)::value;
+      float4 v[S], w[S];
+      if constexpr (GATED) {
+        for (; m < live; m += step, at += step * 512) {
+          ask(s, at, v);
+          ask(s, at + 256, w);
+          const float4 g = add_up(v);
+          finish(code, g, add_up(w));
+        }
+      } else {  // two rows at a time
+        for (; m < live; m += 2 * step, at += 2 * step * 512) {
+          const bool two = m + step < live;
+          ask(s, at, v);
+          if (two) ask(s, at + step * 512, w);
+          finish(code, add_up(v), none);
+          if (two) finish(code, add_up(w), none);
+        }
+      }
+    };
+    auto with_act = [&](auto s) {
+      if (W_MN || p.act == KVS_ACT_NONE) rows(std::integral_constant<int, KVS_ACT_NONE>(), s);  // (dx has none)
+      else if (p.act == KVS_ACT_SILU) rows(std::integral_constant<int, KVS_ACT_SILU>(), s);
+      else if (p.act == KVS_ACT_GELU) rows(std::integral_constant<int, KVS_ACT_GELU>(), s);
+      else rows(std::integral_constant<int, KVS_ACT_RELU>(), s);
+    };
+    if (p.split == 1) with_act(std::integral_constant<int, 1>());
+    else if (p.split == 2) with_act(std::integral_constant<int, 2>());
+    else if (p.split == 4) with_act(std::integral_constant<int, 4>());
+    else with_act(std::integral_constant<int, 8>());
+  }
+  if (p.split > 1) cluster_sync();  // no CTA leaves while another reads its partials
 }
 
 // ------------------------------------------------------------------ gradients of the epilogue
@@ -614,6 +900,25 @@ bool make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int6
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// a [rows][cols] result written in boxes of 32 x 32 (half precision: 64-byte rows, float32: 128)
+bool make_out_map(CUtensorMap* m, void* base, int64_t rows, int64_t cols, int64_t ld, int32_t dtype) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const int size = dtype == KVS_F32 ? 4 : 2;
+  if (rows == 1) ld = (cols + 7) / 8 * 8;  // a single row has no pitch
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * size};
+  const cuuint32_t box[2] = {32, 32};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(m,
+            dtype == KVS_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+            : dtype == KVS_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                               : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+            2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            size == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // An operand of a product: [rows][cols] as it lies in memory.  K-major operands have the reduced
 // index along a row (box of 128 rows), MN-major ones down the rows (two boxes of 64 rows).
 struct Operand {
@@ -655,35 +960,156 @@ template <typename K> int max_pairs(K kernel, KernelState& s) {
   return s.pairs[dev];
 }
 
+// Estimated microseconds of a product on 74 CTA pairs in units of 256 x bn, for choosing between
+// kernels (B200, measured at 512..8192 x 4096 x 4096): about 6 outside the loop, 1.5 a unit, and
+// per K block 0.29 for 256 columns, which the tensor cores bound, but 0.235 for 128, which the
+// 64 bytes per clock that an SM takes from L2 bound (24 KB a block against 32).  Narrow units win
+// where wide ones leave pairs idle: 512 x 4096 x 4096 takes 20.3 us in 64 units of 128 columns,
+// 25.1 in 32 of 256; at 1024 rows it is 35.3 against 27.0.
+double pair_us(int64_t M, int64_t N, int kb, int bn, bool gated) {
+  const int cols = gated ? bn / 2 : bn;
+  const int64_t units = ((M + 255) / 256) * ((N + cols - 1) / cols);
+  return 6.0 + (double)((units + 73) / 74) * (1.5 + kb * (bn == 256 ? 0.29 : 0.235));
+}
+
 struct Product {
   Operand a[2], b[2];
   PairParams p = {};
 };
 
-template <typename T, bool A_MN, bool B_MN, int EPI>
-int launch_pair(const Product& g, int32_t dtype, cudaStream_t st) {
+template <typename T, bool A_MN, bool B_MN, int EPI, int BN>
+int launch_pair_n(const Product& g, int32_t dtype, cudaStream_t st) {
   constexpr bool GATED = EPI == EPI_GATED;
   static KernelState state;
-  const auto kernel = pair_gemm_kernel<T, A_MN, B_MN, EPI>;
+  const auto kernel = pair_gemm_kernel<T, A_MN, B_MN, EPI, BN>;
   const int most = max_pairs(kernel, state);
   if (most <= 0) return KVS_E_UNSUPPORTED;
   CUtensorMap m[4];
   for (int i = 0; i < 2; ++i) {
-    const Operand& a = g.a[i].p ? g.a[i] : g.a[0];
-    const Operand& b = g.b[i].p ? g.b[i] : g.b[0];
-    if (!make_map(&m[i], a.p, a.rows, a.cols, a.ld, A_MN ? 64 : 128, dtype) ||
-        !make_map(&m[2 + i], b.p, b.rows, b.cols, b.ld, B_MN ? 64 : 128, dtype))
-      return KVS_E_UNSUPPORTED;
+    const Operand &a = g.a[i], &b = g.b[i];
+    if (!a.p) m[i] = m[0];  // (no second operand)
+    else if (!make_map(&m[i], a.p, a.rows, a.cols, a.ld, A_MN ? 64 : 128, dtype)) return KVS_E_UNSUPPORTED;
+    if (!b.p) m[2 + i] = m[2];
+    else if (!make_map(&m[2 + i], b.p, b.rows, b.cols, b.ld, B_MN ? 64 : BN / 2, dtype)) return KVS_E_UNSUPPORTED;
   }
   PairParams p = g.p;
+  CUtensorMap o[3] = {m[0], m[0], m[0]};  // (those not written are not used)
+  if (p.vec) {
+    if (!make_out_map(&o[0], p.out0, p.M, p.N, p.ld_out, dtype)) return KVS_E_UNSUPPORTED;
+    if (p.m_parts > 1 && !make_out_map(&o[1], p.out1, p.M, p.N, p.ld_out, dtype)) return KVS_E_UNSUPPORTED;
+    if (p.pre) {  // gate and up have a map each, so that a box at the end of one leaves the other alone
+      const int32_t type = p.pre_f32 ? KVS_F32 : dtype;
+      if (!make_out_map(&o[2], p.pre, p.M, p.N, p.ld_pre, type)) return KVS_E_UNSUPPORTED;
+      uint8_t* up = static_cast<uint8_t*>(p.pre) + (size_t)p.N * (p.pre_f32 ? 4 : 2);
+      if (GATED && !make_out_map(&o[1], up, p.M, p.N, p.ld_pre, type)) return KVS_E_UNSUPPORTED;
+    }
+  }
   p.mb = (p.M + 2 * BM - 1) / (2 * BM);
   p.nb = GATED ? (p.N + BN / 2 - 1) / (BN / 2) : (p.N + BN - 1) / BN;
   const int64_t units = (int64_t)p.mb * p.m_parts * p.nb;
   if (units > (1 << 30)) return KVS_E_UNSUPPORTED;
   p.n_units = (int)units;
   p.group = 8;
-  kernel<<<2 * std::min(most, p.n_units), NT, PAIR_SMEM, st>>>(m[0], m[1], m[2], m[3], p);
+  kernel<<<2 * std::min(most, p.n_units), NT, PAIR_SMEM, st>>>(m[0], m[1], m[2], m[3], o[0], o[1], o[2], p);
   return launch_rc();
+}
+
+// ---- few rows: how a product is cut for the stream kernel
+struct StreamPlan {
+  int tn, stages, split;
+  size_t smem;
+};
+StreamPlan stream_plan(int64_t M, int64_t N, int kb_all, bool gated) {
+  StreamPlan s;
+  const int most = 128;  // rows per tile
+  const int64_t mt = (M + most - 1) / most;
+  s.tn = (int)(((M + mt - 1) / mt + 15) / 16 * 16);
+  const int stage = TILE_BYTES + s.tn * BK * 2;
+  const int parts = s.tn * 128 * 4;  // the partial sums reuse the ring
+  const int fixed = S_BAR_BYTES + 1024;
+  int room = HALF_SM_SMEM - fixed, per_sm = 2;
+  if (room / stage * stage < parts) {
+    room = 232448 - fixed;
+    per_sm = 1;
+  }
+  s.stages = std::min(room / stage, SMAX_STAGES);
+  const int64_t tiles = ((N + (gated ? 63 : 127)) / (gated ? 64 : 128)) * mt;
+  // (powers of two: clusters of other sizes pack badly into the GPCs; 1 x 6144 x 4096 took 18.6 us
+  // with six CTAs a tile, 13.4 us with four)
+  s.split = 1;
+  while (s.split < SMAX_SPLIT && tiles * s.split * 2 <= per_sm * 148 && kb_all / (s.split * 2) >= 2) s.split *= 2;
+  s.smem = (size_t)s.stages * stage + fixed;
+  return s;
+}
+
+template <typename T, bool W_MN, bool GATED>
+int launch_stream(const Operand (&w)[2], const Operand (&x)[2], StreamParams p, int32_t dtype, cudaStream_t st) {
+  static bool set[64] = {};
+  const auto kernel = stream_gemm_kernel<T, W_MN, GATED>;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return KVS_E_UNSUPPORTED;
+  {
+    std::lock_guard<std::mutex> lock(g_mu);
+    if (!set[dev]) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess) {
+        cudaGetLastError();
+        return KVS_E_UNSUPPORTED;
+      }
+      set[dev] = true;
+    }
+  }
+  const StreamPlan s = stream_plan(p.M, p.N, p.n_kb * p.k_parts, GATED);
+  CUtensorMap m[4];
+  for (int i = 0; i < 2; ++i) {
+    if (!w[i].p) m[i] = m[0];  // (no second operand)
+    else if (!make_map(&m[i], w[i].p, w[i].rows, w[i].cols, w[i].ld, W_MN || GATED ? 64 : 128, dtype))
+      return KVS_E_UNSUPPORTED;
+    if (!x[i].p) m[2 + i] = m[2];
+    else if (!make_map(&m[2 + i], x[i].p, x[i].rows, x[i].cols, x[i].ld, s.tn, dtype)) return KVS_E_UNSUPPORTED;
+  }
+  p.tn = s.tn;
+  p.stages = s.stages;
+  p.split = s.split;
+  p.lsplit = s.split == 8 ? 3 : s.split / 2;  // 1, 2, 4, 8
+  p.nt = (p.N + (GATED ? 63 : 127)) / (GATED ? 64 : 128);
+  const int64_t ctas = (int64_t)p.nt * ((p.M + s.tn - 1) / s.tn) * s.split;
+  if (ctas > (1 << 30)) return KVS_E_UNSUPPORTED;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(SNT);
+  cfg.dynamicSmemBytes = s.smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = s.split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, m[0], m[1], m[2], m[3], p);
+  return launch_rc();
+}
+
+template <typename T, bool A_MN, bool B_MN, int EPI>
+int launch_pair(const Product& g, int32_t dtype, cudaStream_t st) {
+  constexpr bool gated = EPI == EPI_GATED;
+  const int64_t m = (int64_t)g.p.M * g.p.m_parts;
+  const int kb = g.p.n_kb * g.p.k_parts;
+  if (pair_us(m, g.p.N, kb, 128, gated) < pair_us(m, g.p.N, kb, 256, gated))
+    return launch_pair_n<T, A_MN, B_MN, EPI, 128>(g, dtype, st);
+  return launch_pair_n<T, A_MN, B_MN, EPI, 256>(g, dtype, st);
+}
+
+// Whether a product of M rows goes to the stream kernel.  Up to 128 rows the weights' bytes bound
+// it (128 x 14336 gated x 4096: 48.1 us against 57 in pair units; 64 x 4096 x 14336: 27.4 against
+// 62).  Beyond, the estimate of what its SMs take from L2 (115 GB/s each) plus finishing decides:
+// 256 x 4096 x 4096 takes 19.1 us here, 22.6 in pairs; 512 x 4096 x 4096 25.6 here, 21.6 in pairs.
+bool use_stream(int64_t M, int64_t N, int kb_all, bool gated) {
+  if (M <= 128) return true;
+  const StreamPlan s = stream_plan(M, N, kb_all, gated);
+  const int64_t ctas = ((N + (gated ? 63 : 127)) / (gated ? 64 : 128)) * ((M + s.tn - 1) / s.tn) * s.split;
+  const double per_sm = (double)((ctas + 147) / 148);
+  const double us = 6.5 + per_sm * ((kb_all + s.split - 1) / s.split * (TILE_BYTES + s.tn * BK * 2) / 115e3 + s.tn * 0.02);
+  return us < std::min(pair_us(M, N, kb_all, 128, gated), pair_us(M, N, kb_all, 256, gated));
 }
 
 bool act_ok(int32_t a) { return a >= KVS_ACT_NONE && a <= KVS_ACT_GELU; }
@@ -724,9 +1150,24 @@ template <typename T> int forward(const kvs_linear_args* a, cudaStream_t st) {
   p.ld_out = a->ld_out;
   p.ld_res = a->ld_res;
   p.ld_pre = a->ld_pre;
-  p.vec = a->n % 4 == 0 && a->ld_out % 4 == 0 && al(a->out, 8) && al(a->bias, 8) && (!a->residual || (a->ld_res % 4 == 0 && al(a->residual, 8))) &&
-          (!a->pre || (a->ld_pre % 4 == 0 && al(a->pre, a->pre_dtype == KVS_F32 ? 16 : 8)));
-  return a->weight_up ? launch_pair<T, false, false, EPI_GATED>(g, a->dtype, st)
+  auto fits = [&](int e) {  // e elements at a time, everywhere
+    const int bytes = 2 * e;
+    return a->n % e == 0 && a->ld_out % e == 0 && al(a->out, bytes) && al(a->bias, bytes) &&
+           (!a->residual || (a->ld_res % e == 0 && al(a->residual, bytes))) &&
+           (!a->pre || (a->ld_pre % e == 0 && al(a->pre, 16)));
+  };
+  const bool gated = a->weight_up != nullptr;
+  if (use_stream(a->rows, a->n, p.n_kb, gated)) {
+    StreamParams s = {};
+    s.M = p.M, s.N = p.N, s.n_kb = p.n_kb, s.k_parts = 1;
+    s.act = p.act, s.vec = fits(4), s.pre_f32 = p.pre_f32;
+    s.out = p.out0, s.bias = p.bias, s.res = p.res, s.pre = p.pre;
+    s.ld_out = p.ld_out, s.ld_res = p.ld_res, s.ld_pre = p.ld_pre;
+    return gated ? launch_stream<T, false, true>(g.b, g.a, s, a->dtype, st)
+                 : launch_stream<T, false, false>(g.b, g.a, s, a->dtype, st);
+  }
+  p.vec = fits(8);
+  return gated ? launch_pair<T, false, false, EPI_GATED>(g, a->dtype, st)
                       : launch_pair<T, false, false, EPI_LINEAR>(g, a->dtype, st);
 }
 
@@ -797,8 +1238,16 @@ template <typename T, typename Z> int backward(const kvs_linear_args* a, const k
     x.p.m_parts = 1;
     x.p.out0 = g->dx;
     x.p.ld_out = g->ld_dx;
-    x.p.vec = g->ld_dx % 4 == 0 && al(g->dx, 8);
-    if ((rc = launch_pair<T, false, true, EPI_STORE>(x, a->dtype, st))) return rc;
+    x.p.vec = g->ld_dx % 8 == 0 && al(g->dx, 16);  // (K is a multiple of 8)
+    if (use_stream(M, K, x.p.n_kb * x.p.k_parts, false)) {
+      StreamParams s = {};
+      s.M = M, s.N = K, s.n_kb = x.p.n_kb, s.k_parts = x.p.k_parts;
+      s.vec = g->ld_dx % 4 == 0 && al(g->dx, 8), s.out = g->dx, s.ld_out = g->ld_dx;
+      rc = launch_stream<T, true, false>(x.b, x.a, s, a->dtype, st);
+    } else {
+      rc = launch_pair<T, false, true, EPI_STORE>(x, a->dtype, st);
+    }
+    if (rc) return rc;
   }
   if (g->dw) {  // [N][K] = dz^T [N][M] x [M][K], summed over the rows (two results when gated)
     Product w;
@@ -813,7 +1262,7 @@ template <typename T, typename Z> int backward(const kvs_linear_args* a, const k
     w.p.out0 = g->dw;
     w.p.out1 = g->dw_up;
     w.p.ld_out = g->ld_dw;
-    w.p.vec = g->ld_dw % 4 == 0 && al(g->dw, 8) && al(g->dw_up, 8);
+    w.p.vec = g->ld_dw % 8 == 0 && al(g->dw, 16) && al(g->dw_up, 16);
     if ((rc = launch_pair<T, true, true, EPI_STORE>(w, a->dtype, st))) return rc;
   }
   return KVS_OK;

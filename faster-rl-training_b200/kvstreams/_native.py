@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -207,6 +208,12 @@ class KvsLinearGrads(C.Structure):
     ]
 
 
+# kvs_linear_args / kvs_linear_grads as packed by struct.pack: several times cheaper than filling a
+# ctypes.Structure field by field, on a path whose kernels run for a few microseconds
+LINEAR_ARGS = struct.Struct("7P6q6i")
+LINEAR_GRADS = struct.Struct("6PN3q")
+assert LINEAR_ARGS.size == C.sizeof(KvsLinearArgs) and LINEAR_GRADS.size == C.sizeof(KvsLinearGrads)
+
 ACTIVATION_CODES = {None: 0, "relu": 1, "silu": 2, "gelu": 3}  # kvs_activation
 
 SIGNATURES = {
@@ -301,6 +308,11 @@ def lib() -> C.CDLL:
     if not torch.cuda.is_available():
         raise RuntimeError("kvstreams kernels need a CUDA (sm_100a) device; none is visible")
     return load_library()
+
+
+def launch_lib() -> C.CDLL:
+    """:func:`lib` for a caller that holds CUDA tensors already: a device is there."""
+    return _lib or lib()
 
 
 def check(rc: int, what: str) -> None:

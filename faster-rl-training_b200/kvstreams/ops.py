@@ -456,127 +456,135 @@ def silu_mul_backward(gu: torch.Tensor, grad: torch.Tensor) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------------- layer products
-class _on:
-    """Makes the device of ``t`` current for a launch (nothing to do when it already is)."""
-
-    __slots__ = ("want", "prev")
-
-    def __init__(self, t: torch.Tensor) -> None:
-        self.want = t.device.index
-
-    def __enter__(self) -> None:
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.want:
-            torch.cuda.set_device(self.want)
-
-    def __exit__(self, *exc) -> None:
-        if self.prev != self.want:
-            torch.cuda.set_device(self.prev)
+# These calls run kernels of a few microseconds in a decode step, so their host side is kept short:
+# arguments are packed with struct (not field by field), checks are plain comparisons, and the device
+# is switched only when it is not the current one.
+_HALF = {torch.bfloat16: N.KVS_BF16, torch.float16: N.KVS_F16}
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _matrix(t: torch.Tensor, cols: int) -> torch.Tensor:
-    """``t`` as ``[rows, cols]`` rows that the products' copies can read where they lie (dense
-    columns, a row pitch that is a multiple of 8, a 16-byte aligned base), else a copy."""
+def _launch(t: torch.Tensor, fn, what: str, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of ``t``'s device, which is made current for it."""
+    dev = t.device.index
+    cur = torch.cuda.current_device()
+    if cur == dev:
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        N.check(rc, what)
+
+
+def _matrix(t: torch.Tensor, cols: int):
+    """``(matrix, address, row pitch)`` of ``t`` as ``[rows, cols]`` rows that the products' copies
+    can read where they lie (dense columns, a row pitch that is a multiple of 8, a 16-byte aligned
+    base), else of a copy."""
     if t.dim() != 2:
         t = t.reshape(-1, cols)
-    if t.stride(1) != 1 or t.data_ptr() % 16 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < cols)):
+    ld, one = t.stride()
+    ptr = t.data_ptr()
+    if t.shape[0] <= 1:
+        ld = cols  # a single row has no pitch
+    if one != 1 or ptr % 16 or ld % 8 or ld < cols:
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        return t, t.data_ptr(), cols
+    return t, ptr, ld
+
+
+def _dense_rows(t: torch.Tensor, cols: int):
+    """``(matrix, address, row pitch)`` of ``t`` as ``[rows, cols]`` with dense columns and rows that
+    do not overlap, else of a copy."""
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
+    ld, one = t.stride()
+    if t.shape[0] <= 1:
+        ld = cols
+    if (one != 1 and cols > 1) or ld < cols:
+        t = t.clone(memory_format=torch.contiguous_format)
+        ld = cols
+    return t, t.data_ptr(), ld
+
+
+def _out_rows(name: str, t: torch.Tensor, cols: int):
+    """``(address, row pitch)`` of an output buffer seen as ``[rows, cols]``, never a copy."""
+    t2 = t if t.dim() == 2 else t.view(-1, cols)  # view raises on rows that do not line up
+    ld, one = t2.stride()
+    if t2.shape[0] <= 1:
+        ld = cols
+    if (one != 1 and cols > 1) or ld < cols:
+        raise ValueError(f"{name} needs dense, non-overlapping rows")
+    return t2.data_ptr(), ld
 
 
 def _same(name: str, t: torch.Tensor, like: torch.Tensor, shape) -> None:
-    if t.dtype != like.dtype or t.device != like.device or tuple(t.shape) != tuple(shape):
+    if t.dtype != like.dtype or t.device != like.device or t.shape != shape:
         raise ValueError(f"{name} must be a {like.dtype} tensor of shape {tuple(shape)} on {like.device} "
                          f"(got {t.dtype} {tuple(t.shape)} on {t.device})")
 
 
-def _dense_rows(t: torch.Tensor, cols: int) -> torch.Tensor:
-    """``t`` as ``[rows, cols]`` with dense columns and rows that do not overlap, else a copy."""
-    if t.dim() != 2:
-        t = t.reshape(-1, cols)
-    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _out_rows(name: str, t: torch.Tensor, cols: int) -> torch.Tensor:
-    """An output buffer as ``[rows, cols]`` without copying; raises where that cannot be done."""
-    t2 = t.view(-1, cols) if t.dim() != 2 else t  # view raises on rows that do not line up
-    if (cols > 1 and t2.stride(1) != 1) or (t2.shape[0] > 1 and t2.stride(0) < cols):
-        raise ValueError(f"{name} needs dense, non-overlapping rows")
-    return t2
-
-
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _product_args(x, weight, weight_up, activation):
-    """Checked operands of a product: the C arguments, the matrices they point into."""
+def _product_sizes(x, weight, weight_up, activation):
+    """Checks a product's operands; ``(n, k, dtype code, activation code)``."""
     if not (x.is_cuda and weight.is_cuda):
         _check_cuda(x, weight)
+    code, act = _HALF.get(x.dtype), N.ACTIVATION_CODES.get(activation)
+    if code is None:
+        raise ValueError(f"layer products take bfloat16 or float16 (got {x.dtype})")
+    if act is None:
+        raise ValueError(f"unknown activation {activation!r}: one of {list(N.ACTIVATION_CODES)}")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
     n, k = weight.shape
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"layer products take bfloat16 or float16 (got {x.dtype})")
     if k == 0 or k % 8 or n == 0:
         raise ValueError(f"layer products need an inner size that is a multiple of 8 and outputs (got {n} x {k})")
-    _same("weight", weight, x, (n, k))
-    code = N.ACTIVATION_CODES.get(activation)
-    if code is None:
-        raise ValueError(f"unknown activation {activation!r}: one of {list(N.ACTIVATION_CODES)}")
-    x2, w2 = _matrix(x, k), _matrix(weight, k)
-    a = N.KvsLinearArgs(x=x2.data_ptr(), weight=w2.data_ptr(), ld_x=_ld(x2), ld_w=_ld(w2), rows=x2.shape[0], n=n,
-                        k=k, dtype=N.DTYPE_CODE[x.dtype], activation=code)
-    keep = [x2, w2]
+    if weight.dtype != x.dtype or weight.device != x.device:
+        _same("weight", weight, x, weight.shape)
     if weight_up is not None:
-        _same("w_up", weight_up, x, (n, k))
-        u2 = _matrix(weight_up, k)
-        a.weight_up, a.ld_w_up = u2.data_ptr(), _ld(u2)
-        keep.append(u2)
-    return a, keep
+        _same("w_up", weight_up, x, weight.shape)
+    return n, k, code, act
 
 
 def pre_buffer(x: torch.Tensor, width: int, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """Buffer for the pre-activations of a product of ``x``: ``[..., width]``, float32 or, for half
     the memory and one more rounding in the gradients, the type of ``x``."""
-    return torch.empty(*x.shape[:-1], width, dtype=dtype, device=x.device)
+    return x.new_empty(x.shape[:-1] + (width,), dtype=dtype)
 
 
-def _set_pre(a, pre: torch.Tensor, x: torch.Tensor, shape, p2) -> torch.Tensor:
-    if pre.dtype not in (torch.float32, x.dtype) or pre.device != x.device or tuple(pre.shape) != tuple(shape):
+def _check_pre(pre: torch.Tensor, x: torch.Tensor, shape) -> int:
+    if pre.dtype not in (torch.float32, x.dtype) or pre.device != x.device or pre.shape != shape:
         raise ValueError(f"pre must be a float32 or {x.dtype} tensor of shape {tuple(shape)} on {x.device} "
                          f"(got {pre.dtype} {tuple(pre.shape)} on {pre.device})")
-    rows = p2(pre)
-    a.pre, a.ld_pre, a.pre_dtype = rows.data_ptr(), _ld(rows), N.DTYPE_CODE[pre.dtype]
-    return rows
+    return N.DTYPE_CODE[pre.dtype]
 
 
 def _product(x, weight, weight_up, activation, bias, residual, pre, out):
-    a, keep = _product_args(x, weight, weight_up, activation)
-    n, lead = a.n, x.shape[:-1]
+    n, k, code, act = _product_sizes(x, weight, weight_up, activation)
+    x2, xp, ldx = _matrix(x, k)
+    w2, wp, ldw = _matrix(weight, k)
+    shape = x.shape[:-1] + (n,)
     if out is None:
-        out = torch.empty(*lead, n, dtype=x.dtype, device=x.device)
+        out = x.new_empty(shape)
+        op, ldo = out.data_ptr(), n
     else:
-        _same("out", out, x, (*lead, n))
-    o2 = _out_rows("out", out, n)
-    a.out, a.ld_out = o2.data_ptr(), _ld(o2)
+        _same("out", out, x, shape)
+        op, ldo = _out_rows("out", out, n)
+    up = bp = rp = pp = ldu = ldr = ldp = pdt = 0
+    if weight_up is not None:
+        u2, up, ldu = _matrix(weight_up, k)
     if bias is not None:
         _same("bias", bias, x, (n,))
-        b = bias.contiguous()
-        a.bias = b.data_ptr()
-        keep.append(b)
+        bias = bias.contiguous()
+        bp = bias.data_ptr()
     if residual is not None:
-        _same("residual", residual, x, (*lead, n))
-        r2 = _dense_rows(residual, n)
-        a.residual, a.ld_res = r2.data_ptr(), _ld(r2)
-        keep.append(r2)
+        _same("residual", residual, x, shape)
+        r2, rp, ldr = _dense_rows(residual, n)
     if pre is not None:
         width = n if weight_up is None else 2 * n
-        _set_pre(a, pre, x, (*lead, width), lambda p: _out_rows("pre", p, width))
-    with _on(x):
-        N.check(N.lib().kvs_linear(C.byref(a), N.stream_ptr(x.device)), "kvs_linear")
+        pdt = _check_pre(pre, x, x.shape[:-1] + (width,))
+        pp, ldp = _out_rows("pre", pre, width)
+    args = N.LINEAR_ARGS.pack(xp, wp, up, bp, rp, pp, op, ldx, ldw, ldu, ldr, ldp, ldo, x2.shape[0], n, k, code, act,
+                              pdt)
+    _launch(x, N.launch_lib().kvs_linear, "kvs_linear", args)
     return out
 
 
@@ -601,31 +609,38 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
 
 
 def _product_backward(gy, x, weight, weight_up, pre, activation, bias_grad):
-    a, keep = _product_args(x, weight, weight_up, activation)
-    n, k, lead = a.n, a.k, x.shape[:-1]
-    _same("the upstream gradient", gy, x, (*lead, n))
-    g2 = _dense_rows(gy, n)
-    if weight_up is not None or activation is not None:
+    n, k, code, act = _product_sizes(x, weight, weight_up, activation)
+    x2, xp, ldx = _matrix(x, k)
+    w2, wp, ldw = _matrix(weight, k)
+    up = ldu = pp = ldp = pdt = dup = dbp = 0
+    if weight_up is not None:
+        u2, up, ldu = _matrix(weight_up, k)
+    _same("the upstream gradient", gy, x, x.shape[:-1] + (n,))
+    g2, gp, ldg = _dense_rows(gy, n)
+    if weight_up is not None or act:
         if pre is None:
             raise ValueError("the backward of an activation needs the forward's pre buffer")
         width = n if weight_up is None else 2 * n
-        keep.append(_set_pre(a, pre, x, (*lead, width), lambda p: _dense_rows(p, width)))
-    dx = torch.empty(*lead, k, dtype=x.dtype, device=x.device)
-    dw = torch.empty(n, k, dtype=x.dtype, device=x.device)
-    du = torch.empty_like(dw) if weight_up is not None else None
-    db = torch.empty(n, dtype=x.dtype, device=x.device) if bias_grad else None
-    g = N.KvsLinearGrads(gy=g2.data_ptr(), dx=dx.data_ptr(), dw=dw.data_ptr(), ld_gy=_ld(g2), ld_dx=k, ld_dw=k)
-    if du is not None:
-        g.dw_up = du.data_ptr()
-    if db is not None:
-        g.db = db.data_ptr()
-    lib = N.lib()
-    nbytes = int(lib.kvs_linear_backward_scratch_bytes(C.byref(a), C.byref(g)))
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    if scratch is not None:
-        g.scratch, g.scratch_bytes = scratch.data_ptr(), nbytes
-    with _on(x):
-        N.check(lib.kvs_linear_backward(C.byref(a), C.byref(g), N.stream_ptr(x.device)), "kvs_linear_backward")
+        pdt = _check_pre(pre, x, x.shape[:-1] + (width,))
+        p2, pp, ldp = _dense_rows(pre, width)
+    dx = x.new_empty(x.shape)
+    dw = x.new_empty((n, k))
+    du = db = scratch = None
+    if weight_up is not None:
+        du = x.new_empty((n, k))
+        dup = du.data_ptr()
+    if bias_grad:
+        db = x.new_empty((n,))
+        dbp = db.data_ptr()
+    lib = N.launch_lib()
+    args = N.LINEAR_ARGS.pack(xp, wp, up, 0, 0, pp, 0, ldx, ldw, ldu, 0, ldp, 0, x2.shape[0], n, k, code, act, pdt)
+    dxp, dwp = dx.data_ptr(), dw.data_ptr()
+    grads = N.LINEAR_GRADS.pack(gp, dxp, dwp, dup, dbp, 0, 0, ldg, k, k)
+    nbytes = lib.kvs_linear_backward_scratch_bytes(args, grads)
+    if nbytes:
+        scratch = x.new_empty((nbytes,), dtype=torch.uint8)
+        grads = N.LINEAR_GRADS.pack(gp, dxp, dwp, dup, dbp, scratch.data_ptr(), nbytes, ldg, k, k)
+    _launch(x, lib.kvs_linear_backward, "kvs_linear_backward", args, grads)
     return dx, dw, du, db
 
 
@@ -649,7 +664,8 @@ def gated_linear_backward(gh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tenso
 
 # ---------------------------------------------------------------------- distillation
 def _distill_args(logits, ids, teacher):
-    _check_cuda(logits, ids, teacher)
+    if not (logits.is_cuda and ids.is_cuda and teacher.is_cuda):
+        _check_cuda(logits, ids, teacher)
     if logits.dtype not in N.DTYPE_CODE:
         raise ValueError(f"unsupported logits dtype {logits.dtype}")
     if logits.dim() != 2 or logits.shape[1] == 0 or logits.stride(1) != 1:
@@ -678,13 +694,11 @@ def distill(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, temp
     slots has loss 0.  One pass over each row; float32 results (float64 for float64 logits)."""
     logits, i, t, acc = _distill_args(logits, ids, teacher)
     n, vocab = logits.shape
-    loss = torch.empty(n, dtype=acc, device=logits.device)
-    lse = torch.empty(n, dtype=acc, device=logits.device)
-    with _on(logits):
-        rc = N.lib().kvs_distill(logits.data_ptr(), _ld(logits), n, vocab, i.data_ptr(), t.data_ptr(), i.shape[1],
-                                 float(temperature), N.DTYPE_CODE[logits.dtype], loss.data_ptr(), lse.data_ptr(),
-                                 N.stream_ptr(logits.device))
-    N.check(rc, "kvs_distill")
+    loss = logits.new_empty((n,), dtype=acc)
+    lse = logits.new_empty((n,), dtype=acc)
+    _launch(logits, N.launch_lib().kvs_distill, "kvs_distill", logits.data_ptr(), _pitch(logits), n, vocab,
+            i.data_ptr(), t.data_ptr(), i.shape[1], temperature, N.DTYPE_CODE[logits.dtype], loss.data_ptr(),
+            lse.data_ptr())
     return loss, lse
 
 
@@ -702,7 +716,7 @@ def distill_backward(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Ten
             raise ValueError(f"{name} must be [{n}] on {logits.device}")
     l, g = lse.to(acc).contiguous(), grad.to(acc).contiguous()
     if out is None:
-        out = torch.empty(n, vocab, dtype=out_dtype or logits.dtype, device=logits.device)
+        out = logits.new_empty((n, vocab), dtype=out_dtype or logits.dtype)
     elif (tuple(out.shape) != (n, vocab) or out.device != logits.device or out.dtype != (out_dtype or out.dtype)
           or (vocab > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < vocab)):
         raise ValueError(f"out must be [{n}, {vocab}] with dense rows on {logits.device}, of type {out_dtype}")
@@ -710,13 +724,14 @@ def distill_backward(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Ten
         raise ValueError("out may be the logits tensor itself, but not overlap it otherwise")
     if out.dtype not in N.DTYPE_CODE:
         raise ValueError(f"unsupported gradient dtype {out.dtype}")
-    with _on(logits):
-        rc = N.lib().kvs_distill_backward(logits.data_ptr(), _ld(logits), n, vocab, i.data_ptr(), t.data_ptr(),
-                                          i.shape[1], l.data_ptr(), g.data_ptr(), float(temperature),
-                                          N.DTYPE_CODE[logits.dtype], out.data_ptr(), _ld(out),
-                                          N.DTYPE_CODE[out.dtype], N.stream_ptr(logits.device))
-    N.check(rc, "kvs_distill_backward")
+    _launch(logits, N.launch_lib().kvs_distill_backward, "kvs_distill_backward", logits.data_ptr(), _pitch(logits), n,
+            vocab, i.data_ptr(), t.data_ptr(), i.shape[1], l.data_ptr(), g.data_ptr(), temperature,
+            N.DTYPE_CODE[logits.dtype], out.data_ptr(), _pitch(out), N.DTYPE_CODE[out.dtype])
     return out
+
+
+def _pitch(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _span(t: torch.Tensor):
