@@ -10,7 +10,7 @@
   for many sequences at once.
 
 Module and parameter names equal the reference's, so state dicts load unchanged.
-Dense projections stay in PyTorch (cuBLAS); attention, RoPE, every cache operation and, for
+Dense projections stay in PyTorch (cuBLAS) unless :attr:`TinyLM.fused_products` is set; attention, RoPE, every cache operation and, for
 half-precision models, RMSNorm and the MLP's silu(gate) * up are this library's kernels.
 """
 
@@ -24,7 +24,7 @@ from torch import nn
 
 from . import _native
 from . import _native as N
-from . import ops
+from . import functional, ops
 from .config import ModelConfig
 from .ops import ReplayMask
 from .rope import RotaryEmbedding
@@ -118,6 +118,8 @@ class Attention(nn.Module):
         """The fused ``[..., (Hq + 2 Hkv) D]`` q|k|v projection of ``x`` (one GEMM over the
         concatenated projection weights)."""
         w = _fused_weight(self, "_qkv", (self.q_proj.weight, self.k_proj.weight, self.v_proj.weight))
+        if self.__dict__.get("_fused_products") and functional.product_kernels(x, w):
+            return functional.linear(x, w)
         return F.linear(x, w)
 
     def project(self, x: torch.Tensor):
@@ -155,10 +157,17 @@ class Block(nn.Module):
     # Residual updates of rows ``x [N, d_model]``: x + o_proj(a) and x + mlp(mlp_norm(x))
     # (model.py:149-152 order), the output projection and the add as one GEMM.
     def attn_residual(self, x: torch.Tensor, a: torch.Tensor) -> torch.Tensor:
+        if self.__dict__.get("_fused_products") and functional.product_kernels(x, self.attn.o_proj.weight):
+            return functional.linear(a, self.attn.o_proj.weight, residual=x)
         return torch.addmm(x, a, self.attn.o_proj.weight.t())
 
     def mlp_residual(self, x: torch.Tensor) -> torch.Tensor:
         h = self.mlp_norm(x)
+        m = self.mlp
+        if self.__dict__.get("_fused_products") and functional.product_kernels(x, m.gate.weight, m.up.weight,
+                                                                               m.down.weight):
+            # both projections, silu and the product in one launch; the sum in the down product's
+            return functional.linear(functional.gated_linear(h, m.gate.weight, m.up.weight), m.down.weight, residual=x)
         gu = F.linear(h, _fused_weight(self.mlp, "_gate_up", (self.mlp.gate.weight, self.mlp.up.weight)))
         return torch.addmm(x, _silu_mul(gu), self.mlp.down.weight.t())
 
@@ -252,6 +261,22 @@ class TinyLM(nn.Module):
     @attention_dtype.setter
     def attention_dtype(self, dtype: Optional[torch.dtype]) -> None:
         self.__dict__["_attention_dtype"] = dtype
+
+    @property
+    def fused_products(self) -> bool:
+        """Whether half-precision layers run their projections in the library's own products
+        (:mod:`kvstreams.functional`): q|k|v, output projection + residual, gate/up/silu/product in
+        one launch, down projection + residual, and their gradients.  Off by default: the layers
+        then use PyTorch's products, whose results differ by the rounding of gate|up and of the
+        gradients' operands.  Layers of other types or sizes keep PyTorch's products either way."""
+        return bool(self.__dict__.get("_fused_products", False))
+
+    @fused_products.setter
+    def fused_products(self, on: bool) -> None:
+        self.__dict__["_fused_products"] = bool(on)
+        for blk in self.layers:
+            blk.__dict__["_fused_products"] = bool(on)
+            blk.attn.__dict__["_fused_products"] = bool(on)
 
     def num_parameters(self) -> int:
         return sum(p.numel() for p in self.parameters())

@@ -608,7 +608,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
     return _product(x, w_gate, w_up, activation, None, None, pre, out)
 
 
-def _product_backward(gy, x, weight, weight_up, pre, activation, bias_grad):
+def _product_backward(gy, x, weight, weight_up, pre, activation, bias_grad, need_dx, need_dw):
     n, k, code, act = _product_sizes(x, weight, weight_up, activation)
     x2, xp, ldx = _matrix(x, k)
     w2, wp, ldw = _matrix(weight, k)
@@ -623,18 +623,22 @@ def _product_backward(gy, x, weight, weight_up, pre, activation, bias_grad):
         width = n if weight_up is None else 2 * n
         pdt = _check_pre(pre, x, x.shape[:-1] + (width,))
         p2, pp, ldp = _dense_rows(pre, width)
-    dx = x.new_empty(x.shape)
-    dw = x.new_empty((n, k))
-    du = db = scratch = None
-    if weight_up is not None:
-        du = x.new_empty((n, k))
-        dup = du.data_ptr()
+    dx = dw = du = db = scratch = None
+    dxp = dwp = 0
+    if need_dx:
+        dx = x.new_empty(x.shape)
+        dxp = dx.data_ptr()
+    if need_dw:
+        dw = x.new_empty((n, k))
+        dwp = dw.data_ptr()
+        if weight_up is not None:
+            du = x.new_empty((n, k))
+            dup = du.data_ptr()
     if bias_grad:
         db = x.new_empty((n,))
         dbp = db.data_ptr()
     lib = N.launch_lib()
     args = N.LINEAR_ARGS.pack(xp, wp, up, 0, 0, pp, 0, ldx, ldw, ldu, 0, ldp, 0, x2.shape[0], n, k, code, act, pdt)
-    dxp, dwp = dx.data_ptr(), dw.data_ptr()
     grads = N.LINEAR_GRADS.pack(gp, dxp, dwp, dup, dbp, 0, 0, ldg, k, k)
     nbytes = lib.kvs_linear_backward_scratch_bytes(args, grads)
     if nbytes:
@@ -645,20 +649,22 @@ def _product_backward(gy, x, weight, weight_up, pre, activation, bias_grad):
 
 
 def linear_backward(gy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre: Optional[torch.Tensor] = None,
-                    activation: Optional[str] = None, bias_grad: bool = False):
-    """``(dx, dw, db)``: gradients of :func:`linear` for the upstream ``gy`` (``db`` None unless
-    ``bias_grad``; the residual's gradient is ``gy`` itself).  An activation needs the forward's
+                    activation: Optional[str] = None, bias_grad: bool = False, need_dx: bool = True,
+                    need_dw: bool = True):
+    """``(dx, dw, db)``: gradients of :func:`linear` for the upstream ``gy`` (None in the place of one
+    not asked for; the residual's gradient is ``gy`` itself).  An activation needs the forward's
     ``pre``.  ``gy act'(pre)`` is rounded to the operands' type for the products; sums run in
     float32 in a fixed order and are rounded once."""
-    dx, dw, _, db = _product_backward(gy, x, weight, None, pre, activation, bias_grad)
+    dx, dw, _, db = _product_backward(gy, x, weight, None, pre, activation, bias_grad, need_dx, need_dw)
     return dx, dw, db
 
 
 def gated_linear_backward(gh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
-                          pre: torch.Tensor, activation: Optional[str] = "silu"):
+                          pre: torch.Tensor, activation: Optional[str] = "silu", need_dx: bool = True,
+                          need_dw: bool = True):
     """``(dx, dw_gate, dw_up)``: gradients of :func:`gated_linear` for the upstream ``gh`` with the
-    forward's gate|up ``pre``."""
-    dx, dg, du, _ = _product_backward(gh, x, w_gate, w_up, pre, activation, False)
+    forward's gate|up ``pre`` (None in the place of those not asked for)."""
+    dx, dg, du, _ = _product_backward(gh, x, w_gate, w_up, pre, activation, False, need_dx, need_dw)
     return dx, dg, du
 
 
