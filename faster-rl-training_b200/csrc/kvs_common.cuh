@@ -26,6 +26,29 @@ inline int launch_rc() {
   return e == cudaSuccess ? KVS_OK : KVS_E_LAUNCH;
 }
 
+// Host: launch with programmatic stream serialization (the kernel begins with
+// pdl_wait_for_previous() before it touches global memory, so its set-up overlaps the end of the
+// kernel before it) and, when cluster > 0, in clusters of that many CTAs along x.
+template <typename... P, typename... A>
+inline int launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                             unsigned cluster, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  return launch_rc();
+}
+
 // First error wins: status[0] is set once, details only by the thread that set it.
 __device__ __forceinline__ void set_status(int32_t* status, int code, int a, int b, int c) {
   if (atomicCAS(status, 0, code) == 0) {

@@ -108,57 +108,85 @@ template <typename T> __device__ __forceinline__ int head_of(const T* p, int n) 
   return min(h, n);
 }
 
-// Running (max, sum of exp((x - max) / T)) of a thread's share of `n` elements at x: 16-byte loads
-// between the ends, kUnroll of them in flight, one rescale of the sum per batch.
+// The row's sum runs in units of 2^z (e^z for double): z = x c with c = log2(e) / T (1 / T), relative
+// to a reference r that is the rounded c times the largest x so far, so that a term is one
+// multiply-add and one exponential, and joining two sums, s1 2^r1 + s2 2^r2, rescales by the very
+// references their terms were formed with.
+__device__ __forceinline__ float power(float z) { return sm100::ex2_approx(z); }
+__device__ __forceinline__ double power(double z) { return exp(z); }
+__device__ __forceinline__ float log_sum(float r, float s) { return (r + log2f(s)) * 0.69314718055994531f; }
+__device__ __forceinline__ double log_sum(double r, double s) { return r + log(s); }
+
+// the largest of a pack (a NaN is passed over here and caught by the sum)
+__device__ __forceinline__ float pack_max(const Pack<float>& q) {
+  return fmaxf(fmaxf(q.v[0], q.v[1]), fmaxf(q.v[2], q.v[3]));
+}
+__device__ __forceinline__ double pack_max(const Pack<double>& q) { return q.v[1] > q.v[0] ? q.v[1] : q.v[0]; }
+template <typename T2, typename T> __device__ __forceinline__ float pack_max_half(const Pack<T>& q) {
+  const T2* h = reinterpret_cast<const T2*>(&q);
+  const T2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(to_acc<T>(m.x), to_acc<T>(m.y));
+}
+__device__ __forceinline__ float pack_max(const Pack<__nv_bfloat16>& q) { return pack_max_half<__nv_bfloat162>(q); }
+__device__ __forceinline__ float pack_max(const Pack<__half>& q) { return pack_max_half<__half2>(q); }
+
+// s += sum over the pack of power(x c - ref); two partial sums for half of float's adds
+template <typename T> __device__ __forceinline__ void pack_sum(const Pack<T>& q, float c, float ref, float& s0, float& s1) {
+#pragma unroll
+  for (int k = 0; k < Pack<T>::n; k += 2) {
+    float z0, z1;
+    sm100::ffma2(z0, z1, to_acc<T>(q.v[k]), to_acc<T>(q.v[k + 1]), c, -ref);
+    sm100::fadd2(s0, s1, power(z0), power(z1));
+  }
+}
+__device__ __forceinline__ void pack_sum(const Pack<double>& q, double c, double ref, double& s0, double& s1) {
+  s0 += power(q.v[0] * c - ref);
+  s1 += power(q.v[1] * c - ref);
+}
+
+// A thread's share of `n` elements at x: reference r (-inf before anything but -inf came) and sum s.
+// 16-byte loads between the ends, kUnroll of them in flight, one rescale of the sum per batch.
 template <int G, typename T, typename A>
-__device__ void row_lse(const T* __restrict__ x, int n, A c, int tid, A& m, A& s) {
+__device__ void row_lse(const T* __restrict__ x, int n, A c, int tid, A& r, A& s) {
   using P = Pack<T>;
   constexpr int kUnroll = 4;
-  auto one = [&](T e) {
-    const A v = to_acc<T>(e);
-    if (v > m) {
-      s = s * exp_scaled(m - v, c) + A(1);
-      m = v;
-    } else if (v != -INFINITY) {  // (-inf - -inf has no exponential; it adds nothing)
-      s += exp_scaled(v - m, c);
+  auto raise = [&](A xm) {  // the reference for a batch whose largest element is xm
+    const A z = xm * c;
+    if (z > r) {
+      s *= power(r - z);  // (0 the first time)
+      r = z;
     }
+    return r == -INFINITY ? A(0) : r;  // nothing but -inf so far: no inf - inf
+  };
+  auto one = [&](T e) {
+    const A v = to_acc<T>(e), ref = raise(v);
+    s += power(v * c - ref);
   };
   const int head = head_of(x, n);
   const int packs = (n - head) / P::n;
   const P* xp = reinterpret_cast<const P*>(x + head);
-  if (tid < head) one(x[tid]);
-  const int tail = head + packs * P::n + tid;
-  if (tail < n) one(x[tail]);  // fewer than P::n <= G elements
   for (int i0 = tid; i0 < packs; i0 += kUnroll * G) {
     P q[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
       if (i0 + u * G < packs) *reinterpret_cast<uint4*>(&q[u]) = __ldg(reinterpret_cast<const uint4*>(xp + i0 + u * G));
-    A bm = -INFINITY;
+    A bm = pack_max(q[0]);
+#pragma unroll
+    for (int u = 1; u < kUnroll; ++u)
+      if (i0 + u * G < packs) {
+        const A m = pack_max(q[u]);
+        bm = m > bm ? m : bm;
+      }
+    const A ref = raise(bm);
+    A s0 = A(0), s1 = A(0);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-      if (i0 + u * G < packs) {
-#pragma unroll
-        for (int k = 0; k < P::n; ++k) {
-          const A v = to_acc<T>(q[u].v[k]);
-          bm = v > bm ? v : bm;
-        }
-      }
-    if (bm > m) {
-      s *= exp_scaled(m - bm, c);
-      m = bm;
-    }
-    // while nothing but -inf came, a reference of 0 keeps the differences away from inf - inf
-    const A ref = m == -INFINITY ? A(0) : m;
-    A part = A(0);
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (i0 + u * G < packs) {
-#pragma unroll
-        for (int k = 0; k < P::n; ++k) part += exp_scaled(to_acc<T>(q[u].v[k]) - ref, c);
-      }
-    s += part;
+      if (i0 + u * G < packs) pack_sum(q[u], c, ref, s0, s1);
+    s += s0 + s1;
   }
+  if (tid < head) one(x[tid]);
+  const int tail = head + packs * P::n + tid;
+  if (tail < n) one(x[tail]);  // fewer than P::n <= G elements
 }
 
 // Grid: rows / (256 / G) CTAs of one row group each, times `segs` CTAs (one cluster) per row.
@@ -170,6 +198,8 @@ distill_kernel(const T* __restrict__ logits, int64_t ld, int n_rows, int vocab, 
   constexpr int PER = (G == 32 ? kWarpTop : kMaxTop) / G;
   __shared__ A red[3 * (kThreads / 32)];
   __shared__ A part[2];
+  sm100::pdl_let_next_start();
+  sm100::pdl_wait_for_previous();
   const int tid = threadIdx.x % G;
   const int seg = segs > 1 ? (int)(blockIdx.x % segs) : 0;
   const int64_t row = (int64_t)(blockIdx.x / segs) * (kThreads / G) + threadIdx.x / G;
@@ -183,7 +213,9 @@ distill_kernel(const T* __restrict__ logits, int64_t ld, int n_rows, int vocab, 
   }
   Slots<A, PER> slot;
   load_slots<G>(ids + row * top, teacher + row * top, seg == 0 ? top : 0, tid, slot);
-  T xs[PER];
+  A r = -INFINITY, s = A(0);
+  row_lse<G, T, A>(x + beg, len, c, tid, r, s);
+  T xs[PER];  // the named logits, just streamed
   A bad = A(0), tm = -INFINITY;
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
@@ -194,13 +226,11 @@ distill_kernel(const T* __restrict__ logits, int64_t ld, int n_rows, int vocab, 
       else bad = A(1);
     }
   }
-  A m = -INFINITY, s = A(0);
-  row_lse<G, T, A>(x + beg, len, c, tid, m, s);
-  A mx[2] = {m, tm};
+  A mx[2] = {r, tm};
   group_reduce<G, MaxOp>(mx, red);
   tm = mx[1];
   // a thread that saw nothing but -inf has s == 0 and adds nothing; a NaN stays one
-  A sum[3] = {s == A(0) ? A(0) : s * exp_scaled(m - mx[0], c), A(0), bad};
+  A sum[3] = {s == A(0) ? A(0) : s * power(r - mx[0]), A(0), bad};
   A e[PER];
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
@@ -208,12 +238,12 @@ distill_kernel(const T* __restrict__ logits, int64_t ld, int n_rows, int vocab, 
     if (slot.id[u] >= 0) sum[1] += exp_full(e[u]);
   }
   group_reduce<G, SumOp>(sum, red);
-  A mm = mx[0], S = sum[0];
+  A rr = mx[0], S = sum[0];
   if (segs > 1) {  // join the segments in order; the first CTA of the cluster goes on
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     if (threadIdx.x == 0) {
-      part[0] = mm;
+      part[0] = rr;
       part[1] = S;
     }
     cluster.sync();
@@ -221,16 +251,16 @@ distill_kernel(const T* __restrict__ logits, int64_t ld, int n_rows, int vocab, 
       A all = -INFINITY, tot = A(0);
       for (int i = 0; i < segs; ++i) all = MaxOp()(all, cluster.map_shared_rank(part, i)[0]);
       for (int i = 0; i < segs; ++i) {
-        const A* r = cluster.map_shared_rank(part, i);
-        if (r[1] != A(0)) tot += r[1] * exp_scaled(r[0] - all, c);
+        const A* o = cluster.map_shared_rank(part, i);
+        if (o[1] != A(0)) tot += o[1] * power(o[0] - all);
       }
-      mm = all;
+      rr = all;
       S = tot;
     }
     cluster.sync();  // the others' shared memory stays until it is read
     if (seg != 0) return;
   }
-  const A lse = mm * inv_temp + log_full(S);
+  const A lse = log_sum(rr, S);
   const A logz = log_full(sum[1]);
   A term[1] = {A(0)};
 #pragma unroll
@@ -276,6 +306,8 @@ distill_bwd_kernel(const T* logits, int64_t ld, int n_rows, int vocab, const int
   __shared__ A red[2 * (kThreads / 32)];
   __shared__ A sp_all[kThreads / G][TOP];
   __shared__ int sid_all[kThreads / G][TOP];
+  sm100::pdl_let_next_start();
+  sm100::pdl_wait_for_previous();
   const int tid = threadIdx.x % G, group = threadIdx.x / G;
   A* sp = sp_all[group];
   int* sid = sid_all[group];
@@ -385,7 +417,7 @@ distill_bwd_kernel(const T* logits, int64_t ld, int n_rows, int vocab, const int
 
 // Short rows go to warps: below this many bytes a row's own work is shorter than a CTA's barriers.
 constexpr int kWarpRowBytes = 4096;
-template <typename T> bool warp_rows(int vocab, int top, int n_rows) {
+template <typename T> bool warp_rows(int vocab, int top) {
   return (int64_t)vocab * (int64_t)sizeof(T) <= kWarpRowBytes && top <= kWarpTop;
 }
 // CTAs per row: doubled while the rows give the machine less than eight CTAs an SM and a segment
@@ -407,30 +439,13 @@ int launch_fwd(const void* logits, int64_t ld, int32_t n_rows, int32_t vocab, co
   const A* t = static_cast<const A*>(teacher);
   const A inv = (A)(1.0 / temperature), c = log2e_of<A>(1.0 / temperature);
   A *l = static_cast<A*>(loss), *e = static_cast<A*>(lse);
-  if (warp_rows<T>(vocab, top, n_rows)) {
-    constexpr int R = kThreads / 32;
-    distill_kernel<T, A, 32><<<(n_rows + R - 1) / R, kThreads, 0, st>>>(x, ld, n_rows, vocab, ids, t, top, inv, c, 1,
-                                                                       l, e);
-    return launch_rc();
-  }
+  constexpr int R = kThreads / 32;
+  if (warp_rows<T>(vocab, top))
+    return launch_overlapped(distill_kernel<T, A, 32>, (n_rows + R - 1) / R, kThreads, 0, st, 0, x, ld, n_rows, vocab,
+                             ids, t, top, inv, c, 1, l, e);
   const int segs = segments<T>(vocab, n_rows);
-  if (segs == 1) {
-    distill_kernel<T, A, kThreads><<<n_rows, kThreads, 0, st>>>(x, ld, n_rows, vocab, ids, t, top, inv, c, 1, l, e);
-    return launch_rc();
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(n_rows * segs);
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = segs;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, distill_kernel<T, A, kThreads>, x, ld, (int)n_rows, (int)vocab, ids, t, (int)top, inv, c,
-                     segs, l, e);
-  return launch_rc();
+  return launch_overlapped(distill_kernel<T, A, kThreads>, n_rows * segs, kThreads, 0, st, segs > 1 ? segs : 0, x, ld,
+                           n_rows, vocab, ids, t, top, inv, c, segs, l, e);
 }
 
 template <typename T, typename A, typename O>
@@ -441,16 +456,13 @@ int launch_bwd(const void* logits, int64_t ld, int32_t n_rows, int32_t vocab, co
   const A *t = static_cast<const A*>(teacher), *e = static_cast<const A*>(lse), *g = static_cast<const A*>(grad);
   const A inv = (A)(1.0 / temperature), c = log2e_of<A>(1.0 / temperature);
   O* d = static_cast<O*>(dlogits);
-  if (warp_rows<T>(vocab, top, n_rows)) {
-    constexpr int R = kThreads / 32;
-    distill_bwd_kernel<T, A, O, 32><<<(n_rows + R - 1) / R, kThreads, 0, st>>>(x, ld, n_rows, vocab, ids, t, top, e, g,
-                                                                              inv, c, 1, d, ld_out);
-  } else {
-    const int segs = segments<T>(vocab, n_rows);
-    distill_bwd_kernel<T, A, O, kThreads><<<n_rows * segs, kThreads, 0, st>>>(x, ld, n_rows, vocab, ids, t, top, e, g,
-                                                                             inv, c, segs, d, ld_out);
-  }
-  return launch_rc();
+  constexpr int R = kThreads / 32;
+  if (warp_rows<T>(vocab, top))
+    return launch_overlapped(distill_bwd_kernel<T, A, O, 32>, (n_rows + R - 1) / R, kThreads, 0, st, 0, x, ld, n_rows,
+                             vocab, ids, t, top, e, g, inv, c, 1, d, ld_out);
+  const int segs = segments<T>(vocab, n_rows);
+  return launch_overlapped(distill_bwd_kernel<T, A, O, kThreads>, n_rows * segs, kThreads, 0, st, 0, x, ld, n_rows,
+                           vocab, ids, t, top, e, g, inv, c, segs, d, ld_out);
 }
 
 // positive and finite, and so is its reciprocal in the arithmetic's type

@@ -223,6 +223,8 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int kb_all = p.n_kb * p.k_parts;
+  pdl_let_next_start();
+  pdl_wait_for_previous();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -581,6 +583,8 @@ stream_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_let_next_start();
+  pdl_wait_for_previous();
   // this CTA's share of the K blocks
   const int kb_all = p.n_kb * p.k_parts;
   const int kb_beg = (int)((int64_t)kb_all * rank / p.split), kb_end = (int)((int64_t)kb_all * (rank + 1) / p.split);
@@ -785,40 +789,65 @@ template <typename T> __device__ __forceinline__ Vec8<T> load8(const T* p, int n
   return r;
 }
 
+// `f` with the activation as a compile-time constant (chosen inside a loop it would be evaluated
+// in every form for every element)
+template <typename F> __device__ __forceinline__ void with_act_code(int act, F f) {
+  if (act == KVS_ACT_SILU) f(std::integral_constant<int, KVS_ACT_SILU>());
+  else if (act == KVS_ACT_GELU) f(std::integral_constant<int, KVS_ACT_GELU>());
+  else if (act == KVS_ACT_RELU) f(std::integral_constant<int, KVS_ACT_RELU>());
+  else f(std::integral_constant<int, KVS_ACT_NONE>());
+}
+
 // dz = gy act'(pre) (or gy itself) into a row pitch the tensor maps take, and its column sums
 // over a chunk of rows (the bias gradient's partials, added up in chunk order: the bits do not
-// depend on scheduling).  64 x 4 threads: eight columns each, rows in steps of four.
+// depend on scheduling).  64 x 4 threads: eight columns each, rows in steps of four, four steps'
+// loads in flight.  Bound by HBM.
 template <typename T, typename Z>
 __global__ void __launch_bounds__(256)
 dz_kernel(const T* __restrict__ gy, int64_t ld_gy, const Z* __restrict__ pre, int64_t ld_pre, int act,
           T* __restrict__ dz, int64_t ld_dz, float* __restrict__ part, int M, int N, int rows_per, int vec) {
   __shared__ float red[4][512];
+  pdl_let_next_start();
+  pdl_wait_for_previous();
   const int c0 = (blockIdx.x * 64 + threadIdx.x) * 8;
-  const int r_end = min(M, (int)(blockIdx.y + 1) * rows_per);
+  const int r_beg = (int)min((int64_t)M, (int64_t)blockIdx.y * rows_per);
+  const int r_end = (int)min((int64_t)M, ((int64_t)blockIdx.y + 1) * rows_per);
   const int nv = N - c0;
   float sum[8] = {};
-  if (nv > 0) {
-    for (int r = blockIdx.y * rows_per + threadIdx.y; r < r_end; r += 4) {
-      const T* g = gy + (int64_t)r * ld_gy + c0;
-      const Z* z = pre ? pre + (int64_t)r * ld_pre + c0 : nullptr;
-      Vec8<T> o;
-      const Vec8<T> gv = load8(g, nv, vec);
-      Vec8<Z> zv;
-      if (z) zv = load8(z, nv, vec);
+  if (nv > 0)
+    with_act_code(act, [&](auto code) {
+      constexpr int ACT = decltype(code)::value;
+      constexpr int U = 4;
+      for (int r0 = r_beg + threadIdx.y; r0 < r_end; r0 += 4 * U) {
+        Vec8<T> gv[U];
+        Vec8<Z> zv[U];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        float d = to_acc<T>(gv.v[k]);
-        if (z) {
-          float a, da;
-          act_grad_f(to_acc<Z>(zv.v[k]), act, a, da);
-          d *= da;
+        for (int u = 0; u < U; ++u) {
+          const int64_t r = r0 + 4 * u;
+          if (r >= r_end) break;
+          gv[u] = load8(gy + r * ld_gy + c0, nv, vec);
+          if (ACT != KVS_ACT_NONE) zv[u] = load8(pre + r * ld_pre + c0, nv, vec);
         }
-        sum[k] += d;
-        o.v[k] = from_acc<T>(d);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t r = r0 + 4 * u;
+          if (r >= r_end) break;
+          Vec8<T> o;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            float d = to_acc<T>(gv[u].v[k]);
+            if (ACT != KVS_ACT_NONE) {
+              float a, da;
+              act_grad_f(to_acc<Z>(zv[u].v[k]), ACT, a, da);
+              d *= da;
+            }
+            sum[k] += d;
+            o.v[k] = from_acc<T>(d);
+          }
+          if (dz) *reinterpret_cast<Vec8<T>*>(dz + r * ld_dz + c0) = o;  // (its pitch is a multiple of 8)
+        }
       }
-      if (dz) *reinterpret_cast<Vec8<T>*>(dz + (int64_t)r * ld_dz + c0) = o;  // pitch a multiple of 8
-    }
-  }
+    });
   if (!part) return;
 #pragma unroll
   for (int k = 0; k < 8; ++k) red[threadIdx.y][threadIdx.x * 8 + k] = sum[k];
@@ -829,41 +858,61 @@ dz_kernel(const T* __restrict__ gy, int64_t ld_gy, const Z* __restrict__ pre, in
   }
 }
 
+// db[j] = sum of the chunks' partials: thread row y takes chunks y, y + 8, ..., then the eight are
+// added in order
 template <typename T>
-__global__ void bias_grad_kernel(const float* __restrict__ part, T* __restrict__ db, int n_parts, int N) {
-  const int j = blockIdx.x * blockDim.x + threadIdx.x;
-  if (j >= N) return;
+__global__ void __launch_bounds__(256)
+bias_grad_kernel(const float* __restrict__ part, T* __restrict__ db, int n_parts, int N) {
+  __shared__ float red[8][32];
+  pdl_let_next_start();
+  pdl_wait_for_previous();
+  const int j = blockIdx.x * 32 + threadIdx.x;
   float s = 0.f;
-  for (int c = 0; c < n_parts; ++c) s += part[(int64_t)c * N + j];
-  db[j] = from_acc<T>(s);
+  if (j < N) {
+#pragma unroll 8
+    for (int c = threadIdx.y; c < n_parts; c += 8) s += part[(int64_t)c * N + j];
+  }
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && j < N) {
+    float t = red[0][threadIdx.x];
+#pragma unroll
+    for (int y = 1; y < 8; ++y) t += red[y][threadIdx.x];
+    db[j] = from_acc<T>(t);
+  }
 }
 
 // dg = gh u act'(g) and du = gh act(g), eight columns per thread; dgu rows hold dg at 0 and du
-// at `half` (N rounded up to 8), zeros between
+// at `half` (N rounded up to 8), zeros between.  Bound by HBM.
 template <typename T, typename Z>
 __global__ void __launch_bounds__(256)
 gated_dz_kernel(const T* __restrict__ gh, int64_t ld_gh, const Z* __restrict__ pre, int64_t ld_pre, int act,
                 T* __restrict__ dgu, int64_t ld_dgu, int half, int64_t M, int N, int vec) {
+  pdl_let_next_start();
+  pdl_wait_for_previous();
   const int nvec = half / 8;
-  for (int64_t idx = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; idx < M * nvec;
-       idx += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = idx / nvec;
-    const int c0 = (int)(idx - r * nvec) * 8, nv = N - c0;
-    const Z* g = pre + r * ld_pre + c0;
-    const Vec8<Z> gv = load8(g, nv, vec), uv = load8(g + N, nv, vec);
-    const Vec8<T> hv = load8(gh + r * ld_gh + c0, nv, vec);
-    Vec8<T> og, ou;
+  with_act_code(act, [&](auto code) {
+    constexpr int ACT = decltype(code)::value;
+    for (int64_t idx = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; idx < M * nvec;
+         idx += (int64_t)gridDim.x * blockDim.x) {
+      const int64_t r = idx / nvec;
+      const int c0 = (int)(idx - r * nvec) * 8, nv = N - c0;
+      const Z* g = pre + r * ld_pre + c0;
+      const Vec8<Z> gv = load8(g, nv, vec), uv = load8(g + N, nv, vec);
+      const Vec8<T> hv = load8(gh + r * ld_gh + c0, nv, vec);
+      Vec8<T> og, ou;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      float a, da;
-      act_grad_f(to_acc<Z>(gv.v[k]), act, a, da);
-      const float hf = to_acc<T>(hv.v[k]);
-      og.v[k] = from_acc<T>(hf * to_acc<Z>(uv.v[k]) * da);
-      ou.v[k] = from_acc<T>(hf * a);
+      for (int k = 0; k < 8; ++k) {
+        float a, da;
+        act_grad_f(to_acc<Z>(gv.v[k]), ACT, a, da);
+        const float hf = to_acc<T>(hv.v[k]);
+        og.v[k] = from_acc<T>(hf * to_acc<Z>(uv.v[k]) * da);
+        ou.v[k] = from_acc<T>(hf * a);
+      }
+      *reinterpret_cast<Vec8<T>*>(dgu + r * ld_dgu + c0) = og;
+      *reinterpret_cast<Vec8<T>*>(dgu + r * ld_dgu + half + c0) = ou;
     }
-    *reinterpret_cast<Vec8<T>*>(dgu + r * ld_dgu + c0) = og;
-    *reinterpret_cast<Vec8<T>*>(dgu + r * ld_dgu + half + c0) = ou;
-  }
+  });
 }
 
 // ------------------------------------------------------------------ host
@@ -1010,8 +1059,8 @@ int launch_pair_n(const Product& g, int32_t dtype, cudaStream_t st) {
   if (units > (1 << 30)) return KVS_E_UNSUPPORTED;
   p.n_units = (int)units;
   p.group = 8;
-  kernel<<<2 * std::min(most, p.n_units), NT, PAIR_SMEM, st>>>(m[0], m[1], m[2], m[3], o[0], o[1], o[2], p);
-  return launch_rc();
+  return launch_overlapped(kernel, 2 * std::min(most, p.n_units), NT, PAIR_SMEM, st, 0, m[0], m[1], m[2], m[3], o[0], o[1],
+                           o[2], p);
 }
 
 // ---- few rows: how a product is cut for the stream kernel
@@ -1074,19 +1123,7 @@ int launch_stream(const Operand (&w)[2], const Operand (&x)[2], StreamParams p, 
   p.nt = (p.N + (GATED ? 63 : 127)) / (GATED ? 64 : 128);
   const int64_t ctas = (int64_t)p.nt * ((p.M + s.tn - 1) / s.tn) * s.split;
   if (ctas > (1 << 30)) return KVS_E_UNSUPPORTED;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(SNT);
-  cfg.dynamicSmemBytes = s.smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = s.split;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kernel, m[0], m[1], m[2], m[3], p);
-  return launch_rc();
+  return launch_overlapped(kernel, (unsigned)ctas, SNT, s.smem, st, s.split, m[0], m[1], m[2], m[3], p);
 }
 
 template <typename T, bool A_MN, bool B_MN, int EPI>
@@ -1198,9 +1235,10 @@ template <typename T, typename Z> int backward(const kvs_linear_args* a, const k
     const bool vec = N % 8 == 0 && al(gy, 16) && al(pre, 16) && g->ld_gy % 8 == 0 && a->ld_pre % 8 == 0;
     T* dgu = reinterpret_cast<T*>(sp);
     const int64_t work = (int64_t)M * (pitch / 8);
-    gated_dz_kernel<T, Z><<<(unsigned)std::min<int64_t>((work + 255) / 256, 148 * 16), 256, 0, st>>>(
-        gy, g->ld_gy, pre, a->ld_pre, a->activation, dgu, 2 * pitch, (int)pitch, M, N, vec);
-    if ((rc = launch_rc())) return rc;
+    rc = launch_overlapped(gated_dz_kernel<T, Z>, (unsigned)std::min<int64_t>((work + 255) / 256, 148 * 16), 256, 0, st, 0,
+                           gy, g->ld_gy, pre, a->ld_pre, a->activation, dgu, 2 * pitch, (int)pitch, (int64_t)M, N,
+                           (int)vec);
+    if (rc) return rc;
     dz[0] = {dgu, M, N, 2 * pitch};
     dz[1] = {dgu + pitch, M, N, 2 * pitch};
   } else {
@@ -1216,12 +1254,13 @@ template <typename T, typename Z> int backward(const kvs_linear_args* a, const k
       float* part = g->db ? reinterpret_cast<float*>(sp) : nullptr;
       const bool act = a->activation != KVS_ACT_NONE;
       const bool vec = N % 8 == 0 && al(gy, 16) && g->ld_gy % 8 == 0 && (!act || (al(pre, 16) && a->ld_pre % 8 == 0));
-      dz_kernel<T, Z><<<dim3((N + 511) / 512, chunks), dim3(64, 4), 0, st>>>(
-          gy, g->ld_gy, act ? pre : nullptr, a->ld_pre, a->activation, own_dz, pitch, part, M, N, per, vec);
-      if ((rc = launch_rc())) return rc;
+      rc = launch_overlapped(dz_kernel<T, Z>, dim3((N + 511) / 512, chunks), dim3(64, 4), 0, st, 0, gy, g->ld_gy,
+                             act ? pre : nullptr, a->ld_pre, a->activation, own_dz, pitch, part, M, N, per, (int)vec);
+      if (rc) return rc;
       if (part) {
-        bias_grad_kernel<T><<<(N + 255) / 256, 256, 0, st>>>(part, static_cast<T*>(g->db), chunks, N);
-        if ((rc = launch_rc())) return rc;
+        rc = launch_overlapped(bias_grad_kernel<T>, (N + 31) / 32, dim3(32, 8), 0, st, 0, part, static_cast<T*>(g->db),
+                               chunks, N);
+        if (rc) return rc;
       }
     }
   }

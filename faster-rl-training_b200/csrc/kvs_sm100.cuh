@@ -157,6 +157,14 @@ template <uint32_t R> __device__ __forceinline__ void regs_alloc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(R));
 }
 
+// ------------------------------------------------------------------ programmatic dependent launch
+// The next kernel of the stream, if it was launched with programmatic stream serialization, may
+// become resident once every CTA of this one has said so (or left).
+__device__ __forceinline__ void pdl_let_next_start() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+// Wait until the kernels before this one have completed and their writes are visible (nothing to
+// wait for when the launch was an ordinary one).  Before any access to global memory.
+__device__ __forceinline__ void pdl_wait_for_previous() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+
 // ------------------------------------------------------------------ TMA
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
