@@ -74,7 +74,7 @@ template <int G, typename Op, typename A, int N> __device__ __forceinline__ void
   }
 }
 
-// A thread's slots of a row, in registers: loaded before the row is streamed, so that their
+// A thread's slots of a row (PER of them; one where a CTA has a thread for each), in registers: loaded before the row is streamed, so that their
 // latency is behind it.  id < 0: empty.
 template <typename A, int PER>
 struct Slots {
@@ -190,12 +190,11 @@ __device__ void row_lse(const T* __restrict__ x, int n, A c, int tid, A& r, A& s
 }
 
 // Grid: rows / (256 / G) CTAs of one row group each, times `segs` CTAs (one cluster) per row.
-template <typename T, typename A, int G>
+template <typename T, typename A, int G, int PER>
 __global__ void __launch_bounds__(kThreads)
 distill_kernel(const T* __restrict__ logits, int64_t ld, int n_rows, int vocab, const int64_t* __restrict__ ids,
                const A* __restrict__ teacher, int top, A inv_temp, A c, int segs, A* __restrict__ loss,
                A* __restrict__ lse_out) {
-  constexpr int PER = (G == 32 ? kWarpTop : kMaxTop) / G;
   __shared__ A red[3 * (kThreads / 32)];
   __shared__ A part[2];
   sm100::pdl_let_next_start();
@@ -297,12 +296,12 @@ template <typename O, typename A, int N> __device__ __forceinline__ void put(O* 
 
 // dlogits may be the logits themselves.  A CTA writes only its segment, after it has read what it
 // needs of it (the entries that slots name).
-template <typename T, typename A, typename O, int G>
+template <typename T, typename A, typename O, int G, int PER>
 __global__ void __launch_bounds__(kThreads)
 distill_bwd_kernel(const T* logits, int64_t ld, int n_rows, int vocab, const int64_t* __restrict__ ids,
                    const A* __restrict__ teacher, int top, const A* __restrict__ lse_in, const A* __restrict__ grad,
                    A inv_temp, A c, int segs, O* dlogits, int64_t ld_out) {
-  constexpr int TOP = G == 32 ? kWarpTop : kMaxTop, PER = TOP / G;
+  constexpr int TOP = G * PER;  // slots of a row at most
   __shared__ A red[2 * (kThreads / 32)];
   __shared__ A sp_all[kThreads / G][TOP];
   __shared__ int sid_all[kThreads / G][TOP];
@@ -441,11 +440,12 @@ int launch_fwd(const void* logits, int64_t ld, int32_t n_rows, int32_t vocab, co
   A *l = static_cast<A*>(loss), *e = static_cast<A*>(lse);
   constexpr int R = kThreads / 32;
   if (warp_rows<T>(vocab, top))
-    return launch_overlapped(distill_kernel<T, A, 32>, (n_rows + R - 1) / R, kThreads, 0, st, 0, x, ld, n_rows, vocab,
-                             ids, t, top, inv, c, 1, l, e);
+    return launch_overlapped(distill_kernel<T, A, 32, kWarpTop / 32>, (n_rows + R - 1) / R, kThreads, 0, st, 0, x, ld,
+                             n_rows, vocab, ids, t, top, inv, c, 1, l, e);
   const int segs = segments<T>(vocab, n_rows);
-  return launch_overlapped(distill_kernel<T, A, kThreads>, n_rows * segs, kThreads, 0, st, segs > 1 ? segs : 0, x, ld,
-                           n_rows, vocab, ids, t, top, inv, c, segs, l, e);
+  const auto kernel = top <= kThreads ? distill_kernel<T, A, kThreads, 1> : distill_kernel<T, A, kThreads, kMaxTop / kThreads>;
+  return launch_overlapped(kernel, n_rows * segs, kThreads, 0, st, segs > 1 ? segs : 0, x, ld, n_rows, vocab, ids, t,
+                           top, inv, c, segs, l, e);
 }
 
 template <typename T, typename A, typename O>
@@ -458,11 +458,13 @@ int launch_bwd(const void* logits, int64_t ld, int32_t n_rows, int32_t vocab, co
   O* d = static_cast<O*>(dlogits);
   constexpr int R = kThreads / 32;
   if (warp_rows<T>(vocab, top))
-    return launch_overlapped(distill_bwd_kernel<T, A, O, 32>, (n_rows + R - 1) / R, kThreads, 0, st, 0, x, ld, n_rows,
-                             vocab, ids, t, top, e, g, inv, c, 1, d, ld_out);
+    return launch_overlapped(distill_bwd_kernel<T, A, O, 32, kWarpTop / 32>, (n_rows + R - 1) / R, kThreads, 0, st, 0, x,
+                             ld, n_rows, vocab, ids, t, top, e, g, inv, c, 1, d, ld_out);
   const int segs = segments<T>(vocab, n_rows);
-  return launch_overlapped(distill_bwd_kernel<T, A, O, kThreads>, n_rows * segs, kThreads, 0, st, 0, x, ld, n_rows,
-                           vocab, ids, t, top, e, g, inv, c, segs, d, ld_out);
+  const auto kernel = top <= kThreads ? distill_bwd_kernel<T, A, O, kThreads, 1>
+                                      : distill_bwd_kernel<T, A, O, kThreads, kMaxTop / kThreads>;
+  return launch_overlapped(kernel, n_rows * segs, kThreads, 0, st, 0, x, ld, n_rows, vocab, ids, t, top, e, g, inv, c,
+                           segs, d, ld_out);
 }
 
 // positive and finite, and so is its reciprocal in the arithmetic's type

@@ -43,10 +43,11 @@ namespace {
 // ------------------------------------------------------------------ element-wise helpers
 __device__ __forceinline__ float sigmoid_f(float z) { return 1.f / (1.f + __expf(-z)); }
 
+// (the last product is kept out of a multiply-add with the residual, so that every path rounds alike)
 __device__ __forceinline__ float act_f(float z, int act) {
   if (act == KVS_ACT_RELU) return z <= 0.f ? 0.f : z;  // a NaN stays one
-  if (act == KVS_ACT_SILU) return z * sigmoid_f(z);
-  if (act == KVS_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  if (act == KVS_ACT_SILU) return __fmul_rn(z, sigmoid_f(z));
+  if (act == KVS_ACT_GELU) return __fmul_rn(0.5f * z, 1.f + erff(z * 0.70710678118654752f));
   return z;
 }
 
@@ -67,6 +68,15 @@ __device__ __forceinline__ void act_grad_f(float z, int act, float& a, float& da
     a = z;
     da = 1.f;
   }
+}
+
+// `f` with the activation as a compile-time constant (chosen inside a loop it would be evaluated
+// in every form for every element)
+template <typename F> __device__ __forceinline__ void with_act_code(int act, F f) {
+  if (act == KVS_ACT_SILU) f(std::integral_constant<int, KVS_ACT_SILU>());
+  else if (act == KVS_ACT_GELU) f(std::integral_constant<int, KVS_ACT_GELU>());
+  else if (act == KVS_ACT_RELU) f(std::integral_constant<int, KVS_ACT_RELU>());
+  else f(std::integral_constant<int, KVS_ACT_NONE>());
 }
 
 template <typename T> struct alignas(sizeof(T) * 4) Vec4 { T v[4]; };
@@ -416,38 +426,53 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
           T* out = static_cast<T*>(part ? p.out1 : p.out0) + (int64_t)row0 * p.ld_out + col + lane;
           int64_t pi = (int64_t)row0 * p.ld_pre + col + lane;
           if constexpr (GATED) {
+            // rows eight at a time: their shared-memory reads in flight together
+            auto column = [&](auto* to, int64_t ld) {
+#pragma unroll 1
+              for (int r0 = 0; r0 < rows; r0 += 8) {
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] = single(r0 + i);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  if (r0 + i < rows && in) to[(r0 + i) * ld] = from_acc<std::remove_reference_t<decltype(*to)>>(f[i]);
+              }
+            };
             if (pre)
               for (int g = 0; g < 2; ++g) {
                 if (g) exchange(u32);
                 else exchange(v);
-#pragma unroll 1
-                for (int r = 0; r < rows; ++r)
-                  if (in) store_pre1<T>(pre, pi + r * p.ld_pre + g * p.N, single(r), pre_f32);
+                if (pre_f32) column(static_cast<float*>(pre) + pi + g * p.N, p.ld_pre);
+                else column(static_cast<T*>(pre) + pi + g * p.N, p.ld_pre);
               }
+            with_act_code(act, [&](auto code) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(act_f(__uint_as_float(v[j]), act) * __uint_as_float(u32[j]));
+              for (int j = 0; j < 32; ++j)
+                v[j] = __float_as_uint(act_f(__uint_as_float(v[j]), decltype(code)::value) * __uint_as_float(u32[j]));
+            });
             exchange(v);
-#pragma unroll 4
-            for (int r = 0; r < rows; ++r)
-              if (in) out[r * p.ld_out] = from_acc<T>(single(r));
+            column(out, p.ld_out);
           } else {
             exchange(v);
             const float b = bias && in ? to_acc<T>(bias[col + lane]) : 0.f;
             const T* from = res + (int64_t)row0 * p.ld_res + col + lane;
+            with_act_code(act, [&](auto code) {
 #pragma unroll 1
-            for (int r0 = 0; r0 < rows; r0 += 8) {
-              float y[8];
+              for (int r0 = 0; r0 < rows; r0 += 8) {
+                float y[8], z[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) y[i] = res && r0 + i < rows && in ? to_acc<T>(from[(r0 + i) * p.ld_res]) : 0.f;
+                for (int i = 0; i < 8; ++i) y[i] = res && r0 + i < rows && in ? to_acc<T>(from[(r0 + i) * p.ld_res]) : 0.f;
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int r = r0 + i;
-                if (r >= rows || !in) continue;
-                const float z = single(r) + b;
-                if (pre) store_pre1<T>(pre, pi + r * p.ld_pre, z, pre_f32);
-                out[r * p.ld_out] = from_acc<T>(act_f(z, act) + y[i]);
+                for (int i = 0; i < 8; ++i) z[i] = single(r0 + i) + b;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const int r = r0 + i;
+                  if (r >= rows || !in) continue;
+                  if (pre) store_pre1<T>(pre, pi + r * p.ld_pre, z[i], pre_f32);
+                  out[r * p.ld_out] = from_acc<T>(act_f(z[i], decltype(code)::value) + y[i]);
+                }
               }
-            }
+            });
           }
           continue;
         }
@@ -476,10 +501,8 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
             v[j] = __float_as_uint(y);
           }
         };
-        if (EPI == EPI_STORE || act == KVS_ACT_NONE) apply(std::integral_constant<int, KVS_ACT_NONE>());
-        else if (act == KVS_ACT_SILU) apply(std::integral_constant<int, KVS_ACT_SILU>());
-        else if (act == KVS_ACT_GELU) apply(std::integral_constant<int, KVS_ACT_GELU>());
-        else apply(std::integral_constant<int, KVS_ACT_RELU>());
+        if constexpr (EPI == EPI_STORE) apply(std::integral_constant<int, KVS_ACT_NONE>());
+        else with_act_code(act, apply);
         if (res) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -766,10 +789,8 @@ stream_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_const
       }
     };
     auto with_act = [&](auto s) {
-      if (W_MN || p.act == KVS_ACT_NONE) rows(std::integral_constant<int, KVS_ACT_NONE>(), s);  // (dx has none)
-      else if (p.act == KVS_ACT_SILU) rows(std::integral_constant<int, KVS_ACT_SILU>(), s);
-      else if (p.act == KVS_ACT_GELU) rows(std::integral_constant<int, KVS_ACT_GELU>(), s);
-      else rows(std::integral_constant<int, KVS_ACT_RELU>(), s);
+      if constexpr (W_MN) rows(std::integral_constant<int, KVS_ACT_NONE>(), s);  // (dx has none)
+      else with_act_code(p.act, [&](auto code) { rows(code, s); });
     };
     if (p.split == 1) with_act(std::integral_constant<int, 1>());
     else if (p.split == 2) with_act(std::integral_constant<int, 2>());
@@ -787,15 +808,6 @@ template <typename T> __device__ __forceinline__ Vec8<T> load8(const T* p, int n
 #pragma unroll
   for (int k = 0; k < 8; ++k) r.v[k] = k < n ? p[k] : from_acc<T>(0.f);
   return r;
-}
-
-// `f` with the activation as a compile-time constant (chosen inside a loop it would be evaluated
-// in every form for every element)
-template <typename F> __device__ __forceinline__ void with_act_code(int act, F f) {
-  if (act == KVS_ACT_SILU) f(std::integral_constant<int, KVS_ACT_SILU>());
-  else if (act == KVS_ACT_GELU) f(std::integral_constant<int, KVS_ACT_GELU>());
-  else if (act == KVS_ACT_RELU) f(std::integral_constant<int, KVS_ACT_RELU>());
-  else f(std::integral_constant<int, KVS_ACT_NONE>());
 }
 
 // dz = gy act'(pre) (or gy itself) into a row pitch the tensor maps take, and its column sums

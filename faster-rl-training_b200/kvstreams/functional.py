@@ -5,6 +5,10 @@
 launch; :func:`distill` is the loss of logits rows against a teacher's top logits.  Each is one
 autograd node over the pair of kernels in :mod:`kvstreams.ops`; only the gradients that are
 needed are computed, and what an activation's gradient needs is kept in float32.
+
+Capturing a backward pass into a CUDA graph: PyTorch ties the accumulation into a leaf to the stream
+of the leaf's first use, so release every eager graph over the same leaves before the capture (or
+capture :func:`kvstreams.ops.linear_backward` and its like, which are plain launches).
 """
 
 from __future__ import annotations

@@ -557,17 +557,30 @@ def _check_pre(pre: torch.Tensor, x: torch.Tensor, shape) -> int:
     return N.DTYPE_CODE[pre.dtype]
 
 
+def _extent(ptr: int, ld: int, rows: int, cols: int, size: int):
+    return ptr, ptr + ((rows - 1) * ld + cols) * size
+
+
+def _apart(name: str, t, others) -> None:
+    """Raises when the extent of a buffer that is written meets one that is read or written meanwhile."""
+    for o in others:
+        if t[0] < o[1] and o[0] < t[1]:
+            raise ValueError(f"{name} overlaps another operand")
+
+
 def _product(x, weight, weight_up, activation, bias, residual, pre, out):
     n, k, code, act = _product_sizes(x, weight, weight_up, activation)
     x2, xp, ldx = _matrix(x, k)
     w2, wp, ldw = _matrix(weight, k)
+    rows = x2.shape[0]
     shape = x.shape[:-1] + (n,)
-    if out is None:
-        out = x.new_empty(shape)
-        op, ldo = out.data_ptr(), n
-    else:
+    given = out is not None
+    if given:
         _same("out", out, x, shape)
         op, ldo = _out_rows("out", out, n)
+    else:
+        out = x.new_empty(shape)
+        op, ldo = out.data_ptr(), n
     up = bp = rp = pp = ldu = ldr = ldp = pdt = 0
     if weight_up is not None:
         u2, up, ldu = _matrix(weight_up, k)
@@ -582,7 +595,21 @@ def _product(x, weight, weight_up, activation, bias, residual, pre, out):
         width = n if weight_up is None else 2 * n
         pdt = _check_pre(pre, x, x.shape[:-1] + (width,))
         pp, ldp = _out_rows("pre", pre, width)
-    args = N.LINEAR_ARGS.pack(xp, wp, up, bp, rp, pp, op, ldx, ldw, ldu, ldr, ldp, ldo, x2.shape[0], n, k, code, act,
+    if (given or pp) and rows:  # buffers of the caller's: apart from what the kernels read (or a copy of it)
+        read = [_extent(xp, ldx, rows, k, 2), _extent(wp, ldw, n, k, 2)]
+        if up:
+            read.append(_extent(up, ldu, n, k, 2))
+        if bp:
+            read.append((bp, bp + 2 * n))
+        res = _extent(rp, ldr, rows, n, 2)
+        dst = _extent(op, ldo, rows, n, 2)
+        if given:
+            _apart("out", dst, read)
+            if rp and not (rp == op and ldr == ldo):  # the residual itself, element for element, may be the output
+                _apart("out", dst, [res])
+        if pp:
+            _apart("pre", _extent(pp, ldp, rows, width, pre.element_size()), read + [dst] + ([res] if rp else []))
+    args = N.LINEAR_ARGS.pack(xp, wp, up, bp, rp, pp, op, ldx, ldw, ldu, ldr, ldp, ldo, rows, n, k, code, act,
                               pdt)
     _launch(x, N.launch_lib().kvs_linear, "kvs_linear", args)
     return out

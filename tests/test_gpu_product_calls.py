@@ -269,6 +269,19 @@ def test_refusals():
     ):
         with pytest.raises(bad):
             call()
+    # outputs over operands that are read meanwhile (k = n here, so the shapes fit)
+    sq, wide = _rand(7, 64, 64), _rand(8, 6, 64)
+    for call in (
+        lambda: ops.linear(x, sq, out=x),
+        lambda: ops.linear(sq, sq, out=sq),
+        lambda: ops.linear(x, sq, residual=wide[:4], out=wide[1:5]),
+        lambda: ops.gated_linear(x, sq, sq, out=x),
+        lambda: ops.linear(x, sq, out=wide[:4], pre=wide[1:5]),
+        lambda: ops.linear(x, sq, residual=wide[:4], pre=wide[:4]),
+    ):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+    assert ops.linear(x, sq, out=wide[2:]).data_ptr() == wide[2:].data_ptr()
     big = torch.zeros(5, 50, device="cuda")
     with pytest.raises(ValueError, match="overlap"):
         ops.distill_backward(big[:4], ids, t, lse, g, out=big[1:])
