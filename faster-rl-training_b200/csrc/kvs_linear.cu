@@ -1088,17 +1088,27 @@ StreamPlan stream_plan(int64_t M, int64_t N, int kb_all, bool gated) {
   const int stage = TILE_BYTES + s.tn * BK * 2;
   const int parts = s.tn * 128 * 4;  // the partial sums reuse the ring
   const int fixed = S_BAR_BYTES + 1024;
-  int room = HALF_SM_SMEM - fixed, per_sm = 2;
-  if (room / stage * stage < parts) {
-    room = 232448 - fixed;
-    per_sm = 1;
-  }
-  s.stages = std::min(room / stage, SMAX_STAGES);
   const int64_t tiles = ((N + (gated ? 63 : 127)) / (gated ? 64 : 128)) * mt;
   // (powers of two: clusters of other sizes pack badly into the GPCs; 1 x 6144 x 4096 took 18.6 us
   // with six CTAs a tile, 13.4 us with four)
-  s.split = 1;
-  while (s.split < SMAX_SPLIT && tiles * s.split * 2 <= per_sm * 148 && kb_all / (s.split * 2) >= 2) s.split *= 2;
+  auto cut = [&](int per_sm) {
+    int split = 1;
+    while (split < SMAX_SPLIT && tiles * split * 2 <= per_sm * 148 && kb_all / (split * 2) >= 2) split *= 2;
+    return split;
+  };
+  // Two CTAs an SM keep every SM loading; one, with the whole shared memory as its ring, halves the
+  // partial sums that an SM exchanges.  One is better where one CTA a SM fills the machine by itself
+  // and there are enough rows for the exchange to count: 64 x 4096 x 4096 12.1 us against 13.1,
+  // 128 x 4096 x 14336 27.7 against 30.3; but 64 x 6144 x 4096 (96 CTAs) 16.8 against 15.7, and
+  // 1 x 4096 x 14336 22.7 against 22.0.
+  int per_sm = 2;
+  const int64_t alone = tiles * cut(1);
+  if (mt == 1 && s.tn >= 32 && alone <= 148 && alone >= 126) per_sm = 1;
+  int room = HALF_SM_SMEM - fixed;
+  if (room / stage * stage < parts) per_sm = 1;
+  if (per_sm == 1) room = 232448 - fixed;
+  s.stages = std::min(room / stage, SMAX_STAGES);
+  s.split = cut(per_sm);
   s.smem = (size_t)s.stages * stage + fixed;
   return s;
 }
