@@ -28,10 +28,20 @@
 // 256-column accumulators, so the epilogue of one unit overlaps the MMAs of the next.  Persistent
 // grid: pair p takes units p, p + P, ...  Every wait is bounded; after one that ran out the
 // outputs of the units concerned are NaN.
+//
+// Where whole units would leave pairs idle (fewer units than pairs, or a last round that is not
+// full) the last units are cut along the reduced index into equal runs of K blocks, one per pair,
+// in unit order.  A pair that comes into a unit in its middle does that part first and leaves the
+// float32 sums in scratch; the pair that holds the unit's beginning does it last, so the others'
+// sums are there when it needs them, adds them in order and finishes the unit.  Parts wait only for
+// pairs of lower block indexes, which were scheduled before, and a part that is waited for never
+// waits itself.
 #include "kvs_common.cuh"
 #include "kvs_sm100.cuh"
 
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 #include <mutex>
 #include <type_traits>
 
@@ -41,7 +51,8 @@ using namespace kvs::sm100;
 namespace {
 
 // ------------------------------------------------------------------ element-wise helpers
-__device__ __forceinline__ float sigmoid_f(float z) { return 1.f / (1.f + __expf(-z)); }
+// (the approximate quotient is good to an ulp or two; 0 past 2^126, where 1 / (1 + e^-z) is below any half step)
+__device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
 
 // (the last product is kept out of a multiply-add with the residual, so that every path rounds alike)
 __device__ __forceinline__ float act_f(float z, int act) {
@@ -151,6 +162,8 @@ struct PairParams {
   int m_parts;     // 2: two results, (a0, b0) -> out0 and (a1, b0) -> out1
   int group;       // row blocks whose columns are walked together (operand reuse in L2)
   int n_units;
+  int whole;       // units done whole; the others' K blocks are dealt out to cut_pairs pairs
+  int cut_pairs;
   int act;
   int vec;         // N is a multiple of 8 and out, res, pre and bias suit 16-byte accesses and TMA
   int pre_f32;     // pre is float32 (else of the activations' type)
@@ -160,7 +173,36 @@ struct PairParams {
   const void* res;
   void* pre;
   int64_t ld_out, ld_res, ld_pre;
+  float* sums;                // [cut_pairs][2 CTAs][8 warps][4 chunks][8][32 lanes][4]: parts' float32 sums
+  unsigned long long* ready;  // [cut_pairs][2][8]: `token` once the sums are there
+  unsigned long long token;   // of this launch; never that of another
 };
+
+constexpr int SUMS_PER_WARP = 32 * 128;  // floats
+
+// What a pair does, one after the other: K blocks k0 .. k1 of unit u.
+struct Part {
+  int u, k0, k1;
+};
+__device__ __forceinline__ int64_t cut_begin(const PairParams& p, int kb_all, int pair) {
+  return (int64_t)(p.n_units - p.whole) * kb_all * pair / p.cut_pairs;
+}
+// the i-th part of a pair; false past the last
+__device__ __forceinline__ bool part_of(const PairParams& p, int kb_all, int pair, int n_pairs, int i, Part& s) {
+  const int64_t u = pair + (int64_t)i * n_pairs;
+  if (u < p.whole) {
+    s = {(int)u, 0, kb_all};
+    return true;
+  }
+  if (pair >= p.cut_pairs) return false;
+  if (pair < p.whole) i -= (p.whole - 1 - pair) / n_pairs + 1;
+  const int64_t beg = cut_begin(p, kb_all, pair), end = cut_begin(p, kb_all, pair + 1);
+  const int64_t first = beg / kb_all + i;  // among the cut units
+  s.u = p.whole + (int)first;
+  s.k0 = i == 0 ? (int)(beg - first * kb_all) : 0;
+  s.k1 = (int)min((int64_t)kb_all, end - first * kb_all);
+  return s.k0 < s.k1;
+}
 
 // unit -> (result, row block, column block): `group` row blocks x all columns at a time, so that
 // the units in flight read few rows of A and few rows of B
@@ -217,7 +259,8 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + OFF_MISC + 4);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_ctarank();  // 0: the even CTA, which issues the MMAs
-  const int pair = (int)(blockIdx.x >> 1), n_pairs = (int)(gridDim.x >> 1);
+  // (in reverse, so that a part waits for CTAs that were scheduled before its own)
+  const int n_pairs = (int)(gridDim.x >> 1), pair = n_pairs - 1 - (int)(blockIdx.x >> 1);
 
   if (tid == 0) {
     for (int i = 0; i < NBAR; ++i) mbar_init(&bar[i], i == B_ACCE || i == B_ACCE + 1 ? 2 * EPI_WARPS : 1);
@@ -241,20 +284,21 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
       // ---------------------------------------------------------------- producer
       bool ok = true;
       int it = 0;
-      for (int u = pair; ok && u < p.n_units; u += n_pairs) {
+      Part s;
+      for (int i = 0; ok && part_of(p, kb_all, pair, n_pairs, i, s); ++i) {
         int part, mb, nb;
-        unit_of(p, u, part, mb, nb);
+        unit_of(p, s.u, part, mb, nb);
         const int row = mb * 2 * BM + (int)rank * BM;
         const int col = GATED ? nb * (BN / 2) : nb * BN + (int)rank * (BN / 2);
-        for (int k = 0; k < kb_all; ++k, ++it) {
-          const int s = it % STAGES;
-          if (it >= STAGES && !mbar_wait_fast(&bar[B_EMPTY + s], ((it / STAGES) - 1) & 1, abort_flag)) {
+        for (int k = s.k0; k < s.k1; ++k, ++it) {
+          const int slot = it % STAGES;
+          if (it >= STAGES && !mbar_wait_fast(&bar[B_EMPTY + slot], ((it / STAGES) - 1) & 1, abort_flag)) {
             ok = false;
             break;
           }
-          const uint32_t full = mapa_shared(&bar[B_FULL + s], 0);
-          if (rank == 0) mbar_arrive_expect_tx(&bar[B_FULL + s], 2 * STAGE_BYTES);
-          uint8_t* st = smem + s * STAGE_BYTES;
+          const uint32_t full = mapa_shared(&bar[B_FULL + slot], 0);
+          if (rank == 0) mbar_arrive_expect_tx(&bar[B_FULL + slot], 2 * STAGE_BYTES);
+          uint8_t* st = smem + slot * STAGE_BYTES;
           const bool second = k >= p.n_kb;  // of two K parts
           const int kb = second ? k - p.n_kb : k;
           load_tile_pair<A_MN, BM>(st, part || second ? &tm_a1 : &tm_a0, kb, row, full);
@@ -275,8 +319,9 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
       constexpr uint32_t AS = A_MN ? 128 : 2, BS = B_MN ? 128 : 2;  // one K16 step: 2 KB / 32 B (>> 4)
       const uint32_t base = smem_addr(smem);
       bool ok = true;
-      int it = 0, ui = 0;
-      for (int u = pair; ok && u < p.n_units; u += n_pairs, ++ui) {
+      int it = 0;
+      Part part;
+      for (int ui = 0; ok && part_of(p, kb_all, pair, n_pairs, ui, part); ++ui) {
         const int ab = ui & 1;
         if (ui >= 2) {
           ok = __all_sync(0xffffffffu, mbar_wait_fast(&bar[B_ACCE + ab], ((ui >> 1) - 1) & 1, abort_flag));
@@ -284,14 +329,14 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
         }
         tc_fence_after();
         const uint32_t d = tmem + ab * BN;
-        for (int k = 0; k < kb_all; ++k, ++it) {
+        for (int k = part.k0; k < part.k1; ++k, ++it) {
           const int s = it % STAGES;
           ok = __all_sync(0xffffffffu, mbar_wait_fast(&bar[B_FULL + s], (it / STAGES) & 1, abort_flag));
           if (!ok) break;
           tc_fence_after();
           const uint64_t da = operand_desc<A_MN>(base + s * STAGE_BYTES);
           const uint64_t db = operand_desc<B_MN>(base + s * STAGE_BYTES + TILE_BYTES);
-          umma_pair_warp_at<0, 0>(d, da, db, IDESC, k > 0);
+          umma_pair_warp_at<0, 0>(d, da, db, IDESC, k > part.k0);
           umma_pair_warp_at<AS, BS>(d, da, db, IDESC, 1);
           umma_pair_warp_at<2 * AS, 2 * BS>(d, da, db, IDESC, 1);
           umma_pair_warp_at<3 * AS, 3 * BS>(d, da, db, IDESC, 1);
@@ -383,11 +428,11 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
       return f;
     };
     bool dead = false;
-    int ui = 0;
-    for (int u = pair; u < p.n_units; u += n_pairs, ++ui) {
+    Part seg;
+    for (int ui = 0; part_of(p, kb_all, pair, n_pairs, ui, seg); ++ui) {
       const int ab = ui & 1;
       int part, mb, nb;
-      unit_of(p, u, part, mb, nb);
+      unit_of(p, seg.u, part, mb, nb);
       const int row0 = mb * 2 * BM + (int)rank * BM + q * 32;
       const int n0 = nb * (GATED ? BN / 2 : BN) + half * COLS;
       const int rows = min(32, p.M - row0);  // existing rows of this warp (may be none)
@@ -399,11 +444,73 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
         for (int k = 0; k < 4; ++k)
           if (n0 + c * 32 + k * 8 < p.N) rv[k] = *reinterpret_cast<const uint4*>(rp + c * 32 + k * 8);
       };
-      if (res && vec) load_res(0);
+      const bool owner = seg.k0 == 0;
+      if (res && vec && owner) load_res(0);
       if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(&bar[B_ACCF + ab], (ui >> 1) & 1, abort_flag));
       if (dead && lane == 0) *abort_flag = 1;
       tc_fence_after();
       const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + ab * BN + half * COLS;
+      if constexpr (BN == 256) {
+        if (!owner) {  // the unit's beginning is another pair's: leave the sums to it
+          const int slot = (pair * 2 + (int)rank) * EPI_WARPS + w;
+          float4* to = reinterpret_cast<float4*>(p.sums + (int64_t)slot * SUMS_PER_WARP) + lane;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32];
+            if (!dead) {
+              tmem_ld32(GATED ? taddr + (c & 1) * 32 + (c >> 1) * (BN / 2) : taddr + c * 32, v);
+              tmem_wait_ld();
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = 0x7fc00000u;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              __stcg(to + (c * 8 + j) * 32, make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]),
+                                                        __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])));
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive_cluster(acce + ab * 8);
+            __threadfence();
+            st_release_gpu(p.ready + slot, p.token);
+          }
+          continue;
+        }
+      }
+      // the pairs that hold the rest of the unit: pair + 1 .. pair + others
+      int others = 0;
+      if (BN == 256 && seg.k1 < kb_all) {
+        const int64_t unit_end = (int64_t)(seg.u - p.whole + 1) * kb_all;
+        while (pair + others + 1 < p.cut_pairs && cut_begin(p, kb_all, pair + others + 1) < unit_end) ++others;
+        bool there = true;
+        if (lane == 0) {
+          for (int r = 1; there && r <= others; ++r) {
+            const unsigned long long* flag = p.ready + ((pair + r) * 2 + (int)rank) * EPI_WARPS + w;
+            there = false;
+            for (int n = 0; n < (1 << 21) && !there; ++n) there = ld_acquire_gpu(flag) == p.token;  // over a second
+          }
+        }
+        if (!__all_sync(0xffffffffu, there)) dead = true;
+      }
+      const float4* sums = reinterpret_cast<const float4*>(p.sums) +
+                           (int64_t)(((pair + 1) * 2 + (int)rank) * EPI_WARPS + w) * (SUMS_PER_WARP / 4) + lane;
+      auto add_others = [&](uint32_t (&v)[32], int c) {
+        for (int r = 0; r < others; ++r) {
+          const float4* from = sums + (int64_t)r * 2 * EPI_WARPS * (SUMS_PER_WARP / 4) + c * 8 * 32;
+          float4 f[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = __ldcg(from + j * 32);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            v[4 * j] = __float_as_uint(__uint_as_float(v[4 * j]) + f[j].x);
+            v[4 * j + 1] = __float_as_uint(__uint_as_float(v[4 * j + 1]) + f[j].y);
+            v[4 * j + 2] = __float_as_uint(__uint_as_float(v[4 * j + 2]) + f[j].z);
+            v[4 * j + 3] = __float_as_uint(__uint_as_float(v[4 * j + 3]) + f[j].w);
+          }
+        }
+      };
 #pragma unroll 1
       for (int c = 0; c < COLS / 32; ++c) {
         const int col = n0 + c * 32;
@@ -419,6 +526,10 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
           if constexpr (GATED)
 #pragma unroll
             for (int j = 0; j < 32; ++j) u32[j] = 0x7fc00000u;
+        }
+        if (others && !dead) {
+          add_others(v, c);
+          if constexpr (GATED) add_others(u32, c + 2);
         }
         if (!vec) {
           // ------------------------------------------------ a lane per column
@@ -521,7 +632,11 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
       // this thread's TMEM reads are done: release the accumulator to the MMA warp
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(acce + ab * 8);
+      if (lane == 0) {
+        mbar_arrive_cluster(acce + ab * 8);
+        // the flags are left as no launch's token, for a replay of this one
+        for (int r = 1; r <= others; ++r) p.ready[((pair + r) * 2 + (int)rank) * EPI_WARPS + w] = 0;
+      }
     }
     if (lane == 0) bulk_wait_read<0>();  // the boxes have left shared memory before the CTA does
     __syncwarp();
@@ -801,21 +916,35 @@ stream_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_const
 }
 
 // ------------------------------------------------------------------ gradients of the epilogue
-// eight consecutive elements, zeros from the n-th on
-template <typename T> __device__ __forceinline__ Vec8<T> load8(const T* p, int n, bool vec) {
-  if (vec) return *reinterpret_cast<const Vec8<T>*>(p);
+// Eight consecutive elements as they lie in memory: as separate half-precision values they would
+// be unpacked, and waited for, where they are loaded.
+template <typename T> struct alignas(16) Raw8 {
+  uint32_t v[2 * sizeof(T)];
+};
+// zeros from the n-th on
+template <typename T> __device__ __forceinline__ Raw8<T> load8(const T* p, int n, bool vec) {
+  if (vec) return *reinterpret_cast<const Raw8<T>*>(p);
   Vec8<T> r;
 #pragma unroll
   for (int k = 0; k < 8; ++k) r.v[k] = k < n ? p[k] : from_acc<T>(0.f);
-  return r;
+  return *reinterpret_cast<const Raw8<T>*>(&r);
+}
+template <typename T> __device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&f)[8]) {
+  const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] = to_acc<T>(e[k]);
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+  *reinterpret_cast<uint4*>(p) =
+      make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
 }
 
 // dz = gy act'(pre) (or gy itself) into a row pitch the tensor maps take, and its column sums
 // over a chunk of rows (the bias gradient's partials, added up in chunk order: the bits do not
-// depend on scheduling).  64 x 4 threads: eight columns each, rows in steps of four, four steps'
-// loads in flight.  Bound by HBM.
+// depend on scheduling).  64 x 4 threads: eight columns each, rows in steps of four, the loads
+// of two to four steps in flight.  Bound by HBM.
 template <typename T, typename Z>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 dz_kernel(const T* __restrict__ gy, int64_t ld_gy, const Z* __restrict__ pre, int64_t ld_pre, int act,
           T* __restrict__ dz, int64_t ld_dz, float* __restrict__ part, int M, int N, int rows_per, int vec) {
   __shared__ float red[4][512];
@@ -829,34 +958,37 @@ dz_kernel(const T* __restrict__ gy, int64_t ld_gy, const Z* __restrict__ pre, in
   if (nv > 0)
     with_act_code(act, [&](auto code) {
       constexpr int ACT = decltype(code)::value;
-      constexpr int U = 4;
+      constexpr int U = ACT == KVS_ACT_NONE ? 4 : 2;
       for (int r0 = r_beg + threadIdx.y; r0 < r_end; r0 += 4 * U) {
-        Vec8<T> gv[U];
-        Vec8<Z> zv[U];
+        Raw8<T> gv[U];
+        Raw8<Z> zv[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int64_t r = r0 + 4 * u;
-          if (r >= r_end) break;
-          gv[u] = load8(gy + r * ld_gy + c0, nv, vec);
-          if (ACT != KVS_ACT_NONE) zv[u] = load8(pre + r * ld_pre + c0, nv, vec);
+          if (r < r_end) {
+            gv[u] = load8(gy + r * ld_gy + c0, nv, vec);
+            if (ACT != KVS_ACT_NONE) zv[u] = load8(pre + r * ld_pre + c0, nv, vec);
+          }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int64_t r = r0 + 4 * u;
-          if (r >= r_end) break;
-          Vec8<T> o;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            float d = to_acc<T>(gv[u].v[k]);
+          if (r < r_end) {
+            float d[8], z[8];
+            unpack8(gv[u], d);
             if (ACT != KVS_ACT_NONE) {
-              float a, da;
-              act_grad_f(to_acc<Z>(zv[u].v[k]), ACT, a, da);
-              d *= da;
+              unpack8(zv[u], z);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                float a, da;
+                act_grad_f(z[k], ACT, a, da);
+                d[k] *= da;
+              }
             }
-            sum[k] += d;
-            o.v[k] = from_acc<T>(d);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum[k] += d[k];
+            if (dz) store8(dz + r * ld_dz + c0, d);  // (its pitch is a multiple of 8)
           }
-          if (dz) *reinterpret_cast<Vec8<T>*>(dz + r * ld_dz + c0) = o;  // (its pitch is a multiple of 8)
         }
       }
     });
@@ -910,19 +1042,21 @@ gated_dz_kernel(const T* __restrict__ gh, int64_t ld_gh, const Z* __restrict__ p
       const int64_t r = idx / nvec;
       const int c0 = (int)(idx - r * nvec) * 8, nv = N - c0;
       const Z* g = pre + r * ld_pre + c0;
-      const Vec8<Z> gv = load8(g, nv, vec), uv = load8(g + N, nv, vec);
-      const Vec8<T> hv = load8(gh + r * ld_gh + c0, nv, vec);
-      Vec8<T> og, ou;
+      const Raw8<Z> gr = load8(g, nv, vec), ur = load8(g + N, nv, vec);
+      const Raw8<T> hr = load8(gh + r * ld_gh + c0, nv, vec);
+      float gv[8], uv[8], hv[8], og[8], ou[8];
+      unpack8(gr, gv);
+      unpack8(ur, uv);
+      unpack8(hr, hv);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         float a, da;
-        act_grad_f(to_acc<Z>(gv.v[k]), ACT, a, da);
-        const float hf = to_acc<T>(hv.v[k]);
-        og.v[k] = from_acc<T>(hf * to_acc<Z>(uv.v[k]) * da);
-        ou.v[k] = from_acc<T>(hf * a);
+        act_grad_f(gv[k], ACT, a, da);
+        og[k] = hv[k] * uv[k] * da;
+        ou[k] = hv[k] * a;
       }
-      *reinterpret_cast<Vec8<T>*>(dgu + r * ld_dgu + c0) = og;
-      *reinterpret_cast<Vec8<T>*>(dgu + r * ld_dgu + half + c0) = ou;
+      store8(dgu + r * ld_dgu + c0, og);
+      store8(dgu + r * ld_dgu + half + c0, ou);
     }
   });
 }
@@ -1021,25 +1155,62 @@ template <typename K> int max_pairs(K kernel, KernelState& s) {
   return s.pairs[dev];
 }
 
-// Estimated microseconds of a product on 74 CTA pairs in units of 256 x bn, for choosing between
-// kernels (B200, measured at 512..8192 x 4096 x 4096): about 6 outside the loop, 1.5 a unit, and
-// per K block 0.29 for 256 columns, which the tensor cores bound, but 0.235 for 128, which the
-// 64 bytes per clock that an SM takes from L2 bound (24 KB a block against 32).  Narrow units win
-// where wide ones leave pairs idle: 512 x 4096 x 4096 takes 20.3 us in 64 units of 128 columns,
-// 25.1 in 32 of 256; at 1024 rows it is 35.3 against 27.0.
-double pair_us(int64_t M, int64_t N, int kb, int bn, bool gated) {
-  const int cols = gated ? bn / 2 : bn;
-  const int64_t units = ((M + 255) / 256) * ((N + cols - 1) / cols);
-  return 6.0 + (double)((units + 73) / 74) * (1.5 + kb * (bn == 256 ? 0.29 : 0.235));
+// How a product is dealt out to the CTA pairs: unit width, units done whole, pairs that share the
+// K blocks of the others, and the estimate in microseconds by which the cut was chosen (B200,
+// measured at 512..8192 x 4096 x 4096).  About 6 outside the loop, 1.5 a unit, and per K block
+// 0.29 for 256 columns, which the tensor cores bound, but 0.235 for 128, which the 64 bytes per clock
+// that an SM takes from L2 bound (24 KB a block against 32).  Cut units cost about 6 (19 MB of sums
+// written at once) and 3 for each pair whose sums the last one to finish has to add.
+constexpr int PAIRS = 74;  // of a B200's 148 SMs
+struct PairPlan {
+  int bn, whole, cut_pairs;
+  double us;
+  size_t scratch() const { return (size_t)cut_pairs * 2 * EPI_WARPS * (SUMS_PER_WARP * 4 + 8); }
+};
+PairPlan pair_plan(int64_t row_blocks, int64_t N, int kb, bool gated, bool cut_allowed) {
+  auto units_of = [&](int bn) { return row_blocks * ((N + (gated ? bn / 2 : bn) - 1) / (gated ? bn / 2 : bn)); };
+  auto rounds = [](int64_t units) { return (double)((units + PAIRS - 1) / PAIRS); };
+  const int64_t units = units_of(256);
+  PairPlan best = {256, (int)std::min<int64_t>(units, 1 << 30), 0, 6.0 + rounds(units) * (1.5 + kb * 0.29)};
+  const double narrow = 6.0 + rounds(units_of(128)) * (1.5 + kb * 0.235);
+  if (narrow < best.us) best = {128, (int)std::min<int64_t>(units_of(128), 1 << 30), 0, narrow};
+  if (!cut_allowed || units % PAIRS == 0 || units >= (1 << 30)) return best;
+  const int64_t whole = std::max<int64_t>(0, units / PAIRS - 1) * PAIRS, rest = units - whole;
+  auto consider = [&](int64_t pairs, int others) {
+    const double run = (double)rest * kb / pairs;  // K blocks a pair
+    if (run < 4) return;
+    const double us = 6.0 + (double)(whole / PAIRS) * (1.5 + kb * 0.29) + run * 0.29 + 1.5 * (1 + (run > kb)) +
+                      6.0 + 3.0 * others;
+    if (us < best.us) best = {256, (int)whole, (int)pairs, us};
+  };
+  // equal cuts of every unit, or all pairs whatever the cuts come to
+  for (int s = 2; rest < PAIRS && rest * s <= PAIRS; ++s) consider(rest * s, s - 1);
+  consider(PAIRS, rest >= PAIRS ? 1 : (int)((PAIRS + rest - 1) / rest));
+  return best;
+}
+PairPlan pair_plan_of(int64_t M, int m_parts, int64_t N, int kb, bool gated, bool cut_allowed) {
+  return pair_plan((M + 2 * BM - 1) / (2 * BM) * m_parts, N, kb, gated, cut_allowed);
 }
 
 struct Product {
   Operand a[2], b[2];
   PairParams p = {};
+  void* scratch = nullptr;  // for cut units' sums
+  size_t scratch_bytes = 0;
 };
 
+// a value that no other launch of this process has, and that memory does not hold by chance
+unsigned long long launch_token() {
+  static std::atomic<unsigned long long> count{(unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count()};
+  unsigned long long z = count.fetch_add(0x9E3779B97F4A7C15ull) + 0x9E3779B97F4A7C15ull;  // SplitMix64 (Steele, Lea, Flood 2014)
+  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+  z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+  z ^= z >> 31;
+  return z ? z : 1;
+}
+
 template <typename T, bool A_MN, bool B_MN, int EPI, int BN>
-int launch_pair_n(const Product& g, int32_t dtype, cudaStream_t st) {
+int launch_pair_n(const Product& g, const PairPlan& plan, int32_t dtype, cudaStream_t st) {
   constexpr bool GATED = EPI == EPI_GATED;
   static KernelState state;
   const auto kernel = pair_gemm_kernel<T, A_MN, B_MN, EPI, BN>;
@@ -1069,9 +1240,19 @@ int launch_pair_n(const Product& g, int32_t dtype, cudaStream_t st) {
   p.nb = GATED ? (p.N + BN / 2 - 1) / (BN / 2) : (p.N + BN - 1) / BN;
   const int64_t units = (int64_t)p.mb * p.m_parts * p.nb;
   if (units > (1 << 30)) return KVS_E_UNSUPPORTED;
-  p.n_units = (int)units;
+  p.n_units = p.whole = (int)units;
+  p.cut_pairs = 0;
   p.group = 8;
-  return launch_overlapped(kernel, 2 * std::min(most, p.n_units), NT, PAIR_SMEM, st, 0, m[0], m[1], m[2], m[3], o[0], o[1],
+  int pairs = std::min(most, p.n_units);
+  if (BN == 256 && plan.cut_pairs > 0 && most >= PAIRS) {
+    p.whole = plan.whole;
+    p.cut_pairs = plan.cut_pairs;
+    pairs = plan.whole > 0 ? PAIRS : plan.cut_pairs;
+    p.ready = static_cast<unsigned long long*>(g.scratch);
+    p.sums = reinterpret_cast<float*>(p.ready + (size_t)plan.cut_pairs * 2 * EPI_WARPS);
+    p.token = launch_token();
+  }
+  return launch_overlapped(kernel, 2 * pairs, NT, PAIR_SMEM, st, 0, m[0], m[1], m[2], m[3], o[0], o[1],
                            o[2], p);
 }
 
@@ -1150,25 +1331,30 @@ int launch_stream(const Operand (&w)[2], const Operand (&x)[2], StreamParams p, 
 
 template <typename T, bool A_MN, bool B_MN, int EPI>
 int launch_pair(const Product& g, int32_t dtype, cudaStream_t st) {
-  constexpr bool gated = EPI == EPI_GATED;
-  const int64_t m = (int64_t)g.p.M * g.p.m_parts;
-  const int kb = g.p.n_kb * g.p.k_parts;
-  if (pair_us(m, g.p.N, kb, 128, gated) < pair_us(m, g.p.N, kb, 256, gated))
-    return launch_pair_n<T, A_MN, B_MN, EPI, 128>(g, dtype, st);
-  return launch_pair_n<T, A_MN, B_MN, EPI, 256>(g, dtype, st);
+  PairPlan plan = pair_plan_of(g.p.M, g.p.m_parts, g.p.N, g.p.n_kb * g.p.k_parts, EPI == EPI_GATED, true);
+  if (plan.scratch() > g.scratch_bytes)
+    plan = pair_plan_of(g.p.M, g.p.m_parts, g.p.N, g.p.n_kb * g.p.k_parts, EPI == EPI_GATED, false);
+  return plan.bn == 128 ? launch_pair_n<T, A_MN, B_MN, EPI, 128>(g, plan, dtype, st)
+                        : launch_pair_n<T, A_MN, B_MN, EPI, 256>(g, plan, dtype, st);
 }
 
 // Whether a product of M rows goes to the stream kernel.  Up to 128 rows the weights' bytes bound
-// it (128 x 14336 gated x 4096: 48.1 us against 57 in pair units; 64 x 4096 x 14336: 27.4 against
+// it (128 x 14336 gated x 4096: 48.1 us against 57 in pair units; 64 x 4096 x 14336: 25.0 against
 // 62).  Beyond, the estimate of what its SMs take from L2 (115 GB/s each) plus finishing decides:
-// 256 x 4096 x 4096 takes 19.1 us here, 22.6 in pairs; 512 x 4096 x 4096 25.6 here, 21.6 in pairs.
+// 256 x 4096 x 4096 takes 17.7 us here, 22.6 in pairs.
 bool use_stream(int64_t M, int64_t N, int kb_all, bool gated) {
   if (M <= 128) return true;
   const StreamPlan s = stream_plan(M, N, kb_all, gated);
   const int64_t ctas = ((N + (gated ? 63 : 127)) / (gated ? 64 : 128)) * ((M + s.tn - 1) / s.tn) * s.split;
   const double per_sm = (double)((ctas + 147) / 148);
   const double us = 6.5 + per_sm * ((kb_all + s.split - 1) / s.split * (TILE_BYTES + s.tn * BK * 2) / 115e3 + s.tn * 0.02);
-  return us < std::min(pair_us(M, N, kb_all, 128, gated), pair_us(M, N, kb_all, 256, gated));
+  return us < pair_plan_of(M, 1, N, kb_all, gated, true).us;
+}
+
+// scratch of one product for its cut units (0: none)
+size_t product_scratch(int64_t M, int m_parts, int64_t N, int kb_all, bool gated, bool may_stream) {
+  if (may_stream && use_stream(M, N, kb_all, gated)) return 0;
+  return pair_plan_of(M, m_parts, N, kb_all, gated, true).scratch();
 }
 
 bool act_ok(int32_t a) { return a >= KVS_ACT_NONE && a <= KVS_ACT_GELU; }
@@ -1226,6 +1412,8 @@ template <typename T> int forward(const kvs_linear_args* a, cudaStream_t st) {
                  : launch_stream<T, false, false>(g.b, g.a, s, a->dtype, st);
   }
   p.vec = fits(8);
+  g.scratch = a->scratch;
+  g.scratch_bytes = a->scratch && al(a->scratch, 16) ? a->scratch_bytes : 0;
   return gated ? launch_pair<T, false, false, EPI_GATED>(g, a->dtype, st)
                       : launch_pair<T, false, false, EPI_LINEAR>(g, a->dtype, st);
 }
@@ -1244,6 +1432,27 @@ bool needs_dz(const kvs_linear_args* a, const kvs_linear_grads* g) {
   return a->activation != KVS_ACT_NONE || !al(g->gy, 16) || (a->rows > 1 && g->ld_gy % 8);
 }
 
+// the backward's products: K blocks of dx (over n, twice when gated) and of dw (over the rows)
+int dx_blocks(const kvs_linear_args* a) { return (a->n + BK - 1) / BK * (a->weight_up ? 2 : 1); }
+int dw_blocks(const kvs_linear_args* a) { return (a->rows + BK - 1) / BK; }
+// scratch of the larger of the two (they run one after the other)
+size_t backward_product_scratch(const kvs_linear_args* a, const kvs_linear_grads* g) {
+  const size_t x = g->dx ? product_scratch(a->rows, 1, a->k, dx_blocks(a), false, true) : 0;
+  const size_t w = g->dw ? product_scratch(a->n, a->weight_up ? 2 : 1, a->k, dw_blocks(a), false, false) : 0;
+  return std::max(x, w);
+}
+// what lies before it: dz and the bias partials
+size_t backward_front_scratch(const kvs_linear_args* a, const kvs_linear_grads* g) {
+  const size_t pitch = (size_t)up8(a->n);
+  if (a->weight_up) return align_up((size_t)a->rows * 2 * pitch * 2, 256);
+  size_t bytes = needs_dz(a, g) ? align_up((size_t)a->rows * pitch * 2, 256) : 0;
+  if (g->db) {
+    const int per = bias_rows_per(a->rows, a->n);
+    bytes += align_up((size_t)((a->rows + per - 1) / per) * a->n * sizeof(float), 256);
+  }
+  return bytes;
+}
+
 template <typename T, typename Z> int backward(const kvs_linear_args* a, const kvs_linear_grads* g, cudaStream_t st) {
   const bool gated = a->weight_up != nullptr;
   const int M = a->rows, N = a->n, K = a->k;
@@ -1253,6 +1462,9 @@ template <typename T, typename Z> int backward(const kvs_linear_args* a, const k
   const Z* pre = static_cast<const Z*>(a->pre);
   Operand dz[2];
   int rc;
+  const size_t front = backward_front_scratch(a, g);
+  void* const cut = sp + front;
+  const size_t cut_bytes = g->scratch_bytes > front ? g->scratch_bytes - front : 0;
   if (gated) {
     const bool vec = N % 8 == 0 && al(gy, 16) && al(pre, 16) && g->ld_gy % 8 == 0 && a->ld_pre % 8 == 0;
     T* dgu = reinterpret_cast<T*>(sp);
@@ -1288,14 +1500,16 @@ template <typename T, typename Z> int backward(const kvs_linear_args* a, const k
   }
   if (g->dx) {  // [M][K] = dz [M][N] W [N][K], summed over N (twice when gated)
     Product x;
+    x.scratch = cut;
+    x.scratch_bytes = cut_bytes;
     x.a[0] = dz[0];
     x.a[1] = dz[1];
     x.b[0] = {a->weight, N, K, a->ld_w};
     if (gated) x.b[1] = {a->weight_up, N, K, a->ld_w_up};
     x.p.M = M;
     x.p.N = K;
-    x.p.n_kb = (N + BK - 1) / BK;
     x.p.k_parts = gated ? 2 : 1;
+    x.p.n_kb = dx_blocks(a) / x.p.k_parts;
     x.p.m_parts = 1;
     x.p.out0 = g->dx;
     x.p.ld_out = g->ld_dx;
@@ -1312,12 +1526,14 @@ template <typename T, typename Z> int backward(const kvs_linear_args* a, const k
   }
   if (g->dw) {  // [N][K] = dz^T [N][M] x [M][K], summed over the rows (two results when gated)
     Product w;
+    w.scratch = cut;
+    w.scratch_bytes = cut_bytes;
     w.a[0] = dz[0];
     w.a[1] = dz[1];
     w.b[0] = {a->x, M, K, a->ld_x};
     w.p.M = N;
     w.p.N = K;
-    w.p.n_kb = (M + BK - 1) / BK;
+    w.p.n_kb = dw_blocks(a);
     w.p.k_parts = 1;
     w.p.m_parts = gated ? 2 : 1;
     w.p.out0 = g->dw;
@@ -1331,6 +1547,11 @@ template <typename T, typename Z> int backward(const kvs_linear_args* a, const k
 
 }  // namespace
 
+KVS_API size_t kvs_linear_scratch_bytes(const kvs_linear_args* a) {
+  if (!a || a->rows <= 0 || a->n <= 0 || a->k <= 0) return 0;
+  return product_scratch(a->rows, 1, a->n, (a->k + BK - 1) / BK, a->weight_up != nullptr, true);
+}
+
 KVS_API int kvs_linear(const kvs_linear_args* a, kvs_stream_t stream) {
   if (int rc = check_common(a)) return rc;
   const bool gated = a->weight_up != nullptr;
@@ -1343,14 +1564,7 @@ KVS_API int kvs_linear(const kvs_linear_args* a, kvs_stream_t stream) {
 
 KVS_API size_t kvs_linear_backward_scratch_bytes(const kvs_linear_args* a, const kvs_linear_grads* g) {
   if (!a || !g || a->rows <= 0 || a->n <= 0) return 0;
-  const size_t pitch = (size_t)up8(a->n);
-  if (a->weight_up) return (size_t)a->rows * 2 * pitch * 2;
-  size_t bytes = needs_dz(a, g) ? align_up((size_t)a->rows * pitch * 2, 256) : 0;
-  if (g->db) {
-    const int per = bias_rows_per(a->rows, a->n);
-    bytes += (size_t)((a->rows + per - 1) / per) * a->n * sizeof(float);
-  }
-  return bytes;
+  return backward_front_scratch(a, g) + backward_product_scratch(a, g);
 }
 
 KVS_API int kvs_linear_backward(const kvs_linear_args* a, const kvs_linear_grads* g, kvs_stream_t stream) {

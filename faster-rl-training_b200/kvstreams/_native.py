@@ -190,6 +190,8 @@ class KvsLinearArgs(C.Structure):
         ("dtype", C.c_int32),
         ("activation", C.c_int32),
         ("pre_dtype", C.c_int32),
+        ("scratch", C.c_void_p),
+        ("scratch_bytes", C.c_size_t),
     ]
 
 
@@ -210,7 +212,7 @@ class KvsLinearGrads(C.Structure):
 
 # kvs_linear_args / kvs_linear_grads as packed by struct.pack: several times cheaper than filling a
 # ctypes.Structure field by field, on a path whose kernels run for a few microseconds
-LINEAR_ARGS = struct.Struct("7P6q6i")
+LINEAR_ARGS = struct.Struct("7P6q6iPN")
 LINEAR_GRADS = struct.Struct("6PN3q")
 assert LINEAR_ARGS.size == C.sizeof(KvsLinearArgs) and LINEAR_GRADS.size == C.sizeof(KvsLinearGrads)
 
@@ -261,6 +263,7 @@ SIGNATURES = {
     "kvs_lm_head_logprobs_supported": (C.c_int, [_I]),
     "kvs_lm_head_logprobs": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _I, _I, _I, _P, C.c_double, _P, _P, _P, _Z,
                                        _P]),
+    "kvs_linear_scratch_bytes": (_Z, [_P]),
     "kvs_linear": (C.c_int, [_P, _P]),
     "kvs_linear_backward_scratch_bytes": (_Z, [_P, _P]),
     "kvs_linear_backward": (C.c_int, [_P, _P, _P]),

@@ -609,9 +609,15 @@ def _product(x, weight, weight_up, activation, bias, residual, pre, out):
                 _apart("out", dst, [res])
         if pp:
             _apart("pre", _extent(pp, ldp, rows, width, pre.element_size()), read + [dst] + ([res] if rp else []))
-    args = N.LINEAR_ARGS.pack(xp, wp, up, bp, rp, pp, op, ldx, ldw, ldu, ldr, ldp, ldo, rows, n, k, code, act,
-                              pdt)
-    _launch(x, N.launch_lib().kvs_linear, "kvs_linear", args)
+    lib = N.launch_lib()
+    args = (xp, wp, up, bp, rp, pp, op, ldx, ldw, ldu, ldr, ldp, ldo, rows, n, k, code, act, pdt)
+    packed = N.LINEAR_ARGS.pack(*args, 0, 0)
+    if rows > 128:  # (fewer rows never need scratch)
+        nbytes = lib.kvs_linear_scratch_bytes(packed)
+        if nbytes:
+            scratch = x.new_empty((nbytes,), dtype=torch.uint8)
+            packed = N.LINEAR_ARGS.pack(*args, scratch.data_ptr(), nbytes)
+    _launch(x, lib.kvs_linear, "kvs_linear", packed)
     return out
 
 
@@ -665,7 +671,8 @@ def _product_backward(gy, x, weight, weight_up, pre, activation, bias_grad, need
         db = x.new_empty((n,))
         dbp = db.data_ptr()
     lib = N.launch_lib()
-    args = N.LINEAR_ARGS.pack(xp, wp, up, 0, 0, pp, 0, ldx, ldw, ldu, 0, ldp, 0, x2.shape[0], n, k, code, act, pdt)
+    args = N.LINEAR_ARGS.pack(xp, wp, up, 0, 0, pp, 0, ldx, ldw, ldu, 0, ldp, 0, x2.shape[0], n, k, code, act, pdt, 0,
+                              0)
     grads = N.LINEAR_GRADS.pack(gp, dxp, dwp, dup, dbp, 0, 0, ldg, k, k)
     nbytes = lib.kvs_linear_backward_scratch_bytes(args, grads)
     if nbytes:

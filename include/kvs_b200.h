@@ -519,7 +519,13 @@ typedef struct kvs_linear_args {
   int32_t dtype;
   int32_t activation;
   int32_t pre_dtype;
+  void* scratch;        /* optional: kvs_linear_scratch_bytes bytes, 16-byte aligned, contents of no matter */
+  size_t scratch_bytes;
 } kvs_linear_args;
+/* Scratch with which kvs_linear deals a product out evenly where its tiles do not come out even
+ * (0: nothing to gain).  Without it, or with less, the product runs in whole tiles.  Calls that may
+ * overlap on the GPU each need their own. */
+size_t kvs_linear_scratch_bytes(const kvs_linear_args* a);
 int kvs_linear(const kvs_linear_args* a, kvs_stream_t stream);
 
 /* Gradients of kvs_linear for the upstream gradient gy [rows][n]; dx [rows][k], dw and dw_up [n][k],

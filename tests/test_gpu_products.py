@@ -3,12 +3,14 @@ same half-precision inputs.
 
 Tolerances.  A forward output is a float32 sum of k exact products (a bf16 or fp16 product is exact
 in float32) plus bias, activation and residual, rounded once.  The sum's error is at most
-k * 2^-24 * sum|x w| and in practice far less: ACC = 2^-18 * sum|x||w| bounds it for k <= 4096 with
-rounding errors of either sign (64 ulps of the absolute sum), the activations add a few float32 ulps
-(covered by the same term) and the final rounding adds eps / 2 of the value.  A backward output is a
-sum of products of two rounded operands: dz carries half a step of its own (eps / 2) and, with an
+k * 2^-24 * sum|x w| and in practice far less: ACC = 2^-18 * sum|x||w| (64 ulps of the absolute sum)
+bounds it up to k = 14344: one rounding per 16 products, 900 of them, each of a partial sum that the
+random signs keep near sqrt(k) = 120 where the absolute sum is near 0.6 k.  The activations add a few
+float32 ulps (covered by the same term) and the final rounding eps / 2 of the value.  A backward output
+is a sum of products of two rounded operands: dz carries half a step of its own (eps / 2) and, with an
 activation, the rounding of the kept pre-activation (2^-24, or half a step of the operands' type) times
-the activation's curvature; the bound is that share of the absolute sum.  The absolute sums are computed in float64 beside the result."""
+the activation's curvature; the bound is that share of the absolute sum.  The absolute sums are
+computed in float64 beside the result."""
 
 import pytest
 import torch
@@ -22,6 +24,10 @@ ACT = {None: lambda z: z, "relu": torch.relu, "silu": F.silu, "gelu": F.gelu}
 # nearest never crosses: a sum of the other sign would have to be below the smallest subnormal.
 SLOPE = {None: (1.0, 0.0), "relu": (1.0, 0.0), "silu": (1.1, 0.5), "gelu": (1.13, 0.8)}
 ACC = 2.0 ** -18
+
+# enough K blocks and few enough tiles that the last ones are cut among the pairs of CTAs: fewer tiles
+# than pairs, and a round of them over; ragged in every index
+CUT = [(600, 1500, 14344), (520, 1001, 14344), (2560, 2305, 4104), (4000, 2560, 4104), (2560, 2304, 4104)]
 
 
 def _half(dtype):
@@ -130,3 +136,57 @@ def test_gated_linear(rows, n, k, keep_half, act, dtype):
     _near(dx, want[0], og @ ag + ou @ au + (bg @ ag + bu @ au) * ACC, dtype, "dx")
     _near(dwg, want[1], (og.t() + bg.t() * ACC) @ ax, dtype, "dwg")
     _near(dwu, want[2], (ou.t() + bu.t() * ACC) @ ax, dtype, "dwu")
+
+
+@pytest.mark.parametrize("rows,n,k", CUT)
+def test_cut_tiles(rows, n, k):
+    """Products whose last tiles are cut along k: forward with every epilogue part, gated with its
+    pre-activations, and both gradients, against float64; the same bits again, and without scratch
+    (whole tiles: another order of the same sums) within the same bounds."""
+    import ctypes as C
+
+    from kvstreams import _native as N, ops
+
+    dtype = BF = torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(rows + n)
+    x, w, u = _rand(g, rows, k), _rand(g, n, k, scale=0.05), _rand(g, n, k, scale=0.05)
+    b, r, gy = _rand(g, n), _rand(g, rows, n), _rand(g, rows, n)
+    args = N.KvsLinearArgs(x=x.data_ptr(), weight=w.data_ptr(), ld_x=k, ld_w=k, ld_out=n, rows=rows, n=n, k=k,
+                           dtype=N.KVS_BF16)
+    assert N.lib().kvs_linear_scratch_bytes(C.byref(args)) > 0  # this size is cut
+    ax, aw, au, ag = (t.double().abs() for t in (x, w, u, gy))
+    z = x.double() @ w.double().t() + b.double()
+    mass = (ax @ aw.t() + b.double().abs()) * ACC + 2.0 ** -20
+    pre = ops.pre_buffer(x, n)
+    y = ops.linear(x, w, b, r, "silu", pre=pre)
+    _near(pre, z, mass, torch.float32, "pre")
+    _near(y, F.silu(z) + r.double(), mass * 1.2 + 2.0 ** -19, BF, "y")
+    assert torch.equal(y, ops.linear(x, w, b, r, "silu"))
+    plain = torch.empty_like(y)
+    args.out, args.bias, args.residual, args.ld_res = plain.data_ptr(), b.data_ptr(), r.data_ptr(), n
+    args.activation = N.ACTIVATION_CODES["silu"]
+    assert N.lib().kvs_linear(C.byref(args), N.stream_ptr(x.device)) == 0
+    _near(plain, F.silu(z) + r.double(), mass * 1.2 + 2.0 ** -19, BF, "whole tiles")
+    gp = ops.pre_buffer(x, 2 * n)
+    h = ops.gated_linear(x, w, u, pre=gp)
+    zg, zu = x.double() @ w.double().t(), x.double() @ u.double().t()
+    mg, mu = ax @ aw.t() * ACC + 2.0 ** -20, ax @ au.t() * ACC + 2.0 ** -20
+    _near(gp[:, :n], zg, mg, torch.float32, "gate")
+    _near(gp[:, n:], zu, mu, torch.float32, "up")
+    _near(h, F.silu(zg) * zu, 1.1 * mg * (zu.abs() + mu) + (1.1 * zg.abs() + mg) * mu + 2.0 ** -19, BF, "h")
+    assert torch.equal(h, ops.gated_linear(x, w, u))
+    dx, dw, db = ops.linear_backward(gy, x, w, bias_grad=True)
+    gd = gy.double()
+    _near(dx, gd @ w.double(), ag @ aw * ACC, BF, "dx")
+    _near(dw, gd.t() @ x.double(), ag.t() @ ax * ACC, BF, "dw")
+    again = ops.linear_backward(gy, x, w, bias_grad=True)
+    assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), again))
+    gx, g1, g2 = ops.gated_linear_backward(gy, x, w, u, gp)
+    again = ops.gated_linear_backward(gy, x, w, u, gp)
+    assert all(torch.equal(p, q) for p, q in zip((gx, g1, g2), again))
+    s = torch.sigmoid(zg)
+    dg, du = gd * zu * s * (1 + zg * (1 - s)), gd * F.silu(zg)
+    e = 2.0 ** -8 * 1.01  # the rounding of dg and du, and the float32 errors behind it
+    _near(gx, dg @ w.double() + du @ u.double(), e * (dg.abs() @ aw + du.abs() @ au) + 2.0 ** -10, BF, "gated dx")
+    _near(g1, dg.t() @ x.double(), e * dg.abs().t() @ ax + 2.0 ** -10, BF, "dw gate")
+    _near(g2, du.t() @ x.double(), e * du.abs().t() @ ax + 2.0 ** -10, BF, "dw up")
