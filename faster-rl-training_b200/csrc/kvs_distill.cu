@@ -108,15 +108,6 @@ template <typename T> __device__ __forceinline__ int head_of(const T* p, int n) 
   return min(h, n);
 }
 
-// The row's sum runs in units of 2^z (e^z for double): z = x c with c = log2(e) / T (1 / T), relative
-// to a reference r that is the rounded c times the largest x so far, so that a term is one
-// multiply-add and one exponential, and joining two sums, s1 2^r1 + s2 2^r2, rescales by the very
-// references their terms were formed with.
-__device__ __forceinline__ float power(float z) { return sm100::ex2_approx(z); }
-__device__ __forceinline__ double power(double z) { return exp(z); }
-__device__ __forceinline__ float log_sum(float r, float s) { return (r + log2f(s)) * 0.69314718055994531f; }
-__device__ __forceinline__ double log_sum(double r, double s) { return r + log(s); }
-
 // the largest of a pack (a NaN is passed over here and caught by the sum)
 __device__ __forceinline__ float pack_max(const Pack<float>& q) {
   return fmaxf(fmaxf(q.v[0], q.v[1]), fmaxf(q.v[2], q.v[3]));
@@ -130,37 +121,39 @@ template <typename T2, typename T> __device__ __forceinline__ float pack_max_hal
 __device__ __forceinline__ float pack_max(const Pack<__nv_bfloat16>& q) { return pack_max_half<__nv_bfloat162>(q); }
 __device__ __forceinline__ float pack_max(const Pack<__half>& q) { return pack_max_half<__half2>(q); }
 
-// s += sum over the pack of power(x c - ref); two partial sums for half of float's adds
-template <typename T> __device__ __forceinline__ void pack_sum(const Pack<T>& q, float c, float ref, float& s0, float& s1) {
+// s += sum over the pack of exp((x - m) / T); two partial sums, and float's differences, scalings
+// and sums two at a time.  (The difference is formed before it is scaled: x / T log2(e) of a logit
+// at the type's lowest value would overflow, and its rounding would be that of the large number.)
+template <typename T> __device__ __forceinline__ void pack_sum(const Pack<T>& q, float c, float m, float& s0, float& s1) {
 #pragma unroll
   for (int k = 0; k < Pack<T>::n; k += 2) {
     float z0, z1;
-    sm100::ffma2(z0, z1, to_acc<T>(q.v[k]), to_acc<T>(q.v[k + 1]), c, -ref);
-    sm100::fadd2(s0, s1, power(z0), power(z1));
+    sm100::addmul2(z0, z1, to_acc<T>(q.v[k]), to_acc<T>(q.v[k + 1]), -m, -m, c, c);
+    sm100::fadd2(s0, s1, sm100::ex2_approx(z0), sm100::ex2_approx(z1));
   }
 }
-__device__ __forceinline__ void pack_sum(const Pack<double>& q, double c, double ref, double& s0, double& s1) {
-  s0 += power(q.v[0] * c - ref);
-  s1 += power(q.v[1] * c - ref);
+__device__ __forceinline__ void pack_sum(const Pack<double>& q, double c, double m, double& s0, double& s1) {
+  s0 += exp_scaled(q.v[0] - m, c);
+  s1 += exp_scaled(q.v[1] - m, c);
 }
 
-// A thread's share of `n` elements at x: reference r (-inf before anything but -inf came) and sum s.
-// 16-byte loads between the ends, kUnroll of them in flight, one rescale of the sum per batch.
+// A thread's share of `n` elements at x: the largest, m (-inf before anything but -inf came), and
+// s = sum of exp((x - m) / T).  16-byte loads between the ends, kUnroll of them in flight, one
+// rescale of the sum per batch.
 template <int G, typename T, typename A>
-__device__ void row_lse(const T* __restrict__ x, int n, A c, int tid, A& r, A& s) {
+__device__ void row_lse(const T* __restrict__ x, int n, A c, int tid, A& m, A& s) {
   using P = Pack<T>;
   constexpr int kUnroll = 4;
   auto raise = [&](A xm) {  // the reference for a batch whose largest element is xm
-    const A z = xm * c;
-    if (z > r) {
-      s *= power(r - z);  // (0 the first time)
-      r = z;
+    if (xm > m) {
+      s *= exp_scaled(m - xm, c);  // (0 the first time)
+      m = xm;
     }
-    return r == -INFINITY ? A(0) : r;  // nothing but -inf so far: no inf - inf
+    return m == -INFINITY ? A(0) : m;  // nothing but -inf so far: no inf - inf
   };
   auto one = [&](T e) {
     const A v = to_acc<T>(e), ref = raise(v);
-    s += power(v * c - ref);
+    s += exp_scaled(v - ref, c);
   };
   const int head = head_of(x, n);
   const int packs = (n - head) / P::n;
@@ -174,8 +167,8 @@ __device__ void row_lse(const T* __restrict__ x, int n, A c, int tid, A& r, A& s
 #pragma unroll
     for (int u = 1; u < kUnroll; ++u)
       if (i0 + u * G < packs) {
-        const A m = pack_max(q[u]);
-        bm = m > bm ? m : bm;
+        const A pm = pack_max(q[u]);
+        bm = pm > bm ? pm : bm;
       }
     const A ref = raise(bm);
     A s0 = A(0), s1 = A(0);
@@ -212,8 +205,8 @@ distill_kernel(const T* __restrict__ logits, int64_t ld, int n_rows, int vocab, 
   }
   Slots<A, PER> slot;
   load_slots<G>(ids + row * top, teacher + row * top, seg == 0 ? top : 0, tid, slot);
-  A r = -INFINITY, s = A(0);
-  row_lse<G, T, A>(x + beg, len, c, tid, r, s);
+  A m = -INFINITY, s = A(0);
+  row_lse<G, T, A>(x + beg, len, c, tid, m, s);
   T xs[PER];  // the named logits, just streamed
   A bad = A(0), tm = -INFINITY;
 #pragma unroll
@@ -225,11 +218,11 @@ distill_kernel(const T* __restrict__ logits, int64_t ld, int n_rows, int vocab, 
       else bad = A(1);
     }
   }
-  A mx[2] = {r, tm};
+  A mx[2] = {m, tm};
   group_reduce<G, MaxOp>(mx, red);
   tm = mx[1];
   // a thread that saw nothing but -inf has s == 0 and adds nothing; a NaN stays one
-  A sum[3] = {s == A(0) ? A(0) : s * power(r - mx[0]), A(0), bad};
+  A sum[3] = {s == A(0) ? A(0) : s * exp_scaled(m - mx[0], c), A(0), bad};
   A e[PER];
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
@@ -237,12 +230,12 @@ distill_kernel(const T* __restrict__ logits, int64_t ld, int n_rows, int vocab, 
     if (slot.id[u] >= 0) sum[1] += exp_full(e[u]);
   }
   group_reduce<G, SumOp>(sum, red);
-  A rr = mx[0], S = sum[0];
+  A mm = mx[0], S = sum[0];
   if (segs > 1) {  // join the segments in order; the first CTA of the cluster goes on
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     if (threadIdx.x == 0) {
-      part[0] = rr;
+      part[0] = mm;
       part[1] = S;
     }
     cluster.sync();
@@ -251,15 +244,15 @@ distill_kernel(const T* __restrict__ logits, int64_t ld, int n_rows, int vocab, 
       for (int i = 0; i < segs; ++i) all = MaxOp()(all, cluster.map_shared_rank(part, i)[0]);
       for (int i = 0; i < segs; ++i) {
         const A* o = cluster.map_shared_rank(part, i);
-        if (o[1] != A(0)) tot += o[1] * power(o[0] - all);
+        if (o[1] != A(0)) tot += o[1] * exp_scaled(o[0] - all, c);
       }
-      rr = all;
+      mm = all;
       S = tot;
     }
     cluster.sync();  // the others' shared memory stays until it is read
     if (seg != 0) return;
   }
-  const A lse = log_sum(rr, S);
+  const A lse = mm * inv_temp + log_full(S);
   const A logz = log_full(sum[1]);
   A term[1] = {A(0)};
 #pragma unroll

@@ -112,6 +112,27 @@ def test_masked_vocabulary():
     assert ops.distill(x, ids, t)[0][1].isnan()
 
 
+def test_whole_segments_masked():
+    """Rows whose threads, batches or cluster segments see nothing but masked logits (one entry is
+    left): lse is that entry, its probability 1.  A row of -inf only has no distribution: NaN."""
+    from kvstreams import ops
+
+    for vocab in (1000, 40000, 128256):
+        for low in (-math.inf, torch.finfo(torch.float32).min):
+            for at in (0, vocab // 2, vocab - 1):
+                x = torch.full((2, vocab), low, device="cuda")
+                x[:, at] = 3.0
+                ids = torch.full((2, 1), at, dtype=torch.long, device="cuda")
+                t = torch.zeros(2, 1, device="cuda")
+                loss, lse = ops.distill(x, ids, t)
+                assert (lse == 3.0).all() and (loss == 0).all()
+                d = ops.distill_backward(x, ids, t, lse, torch.ones(2, device="cuda"))
+                assert (d == 0).all()  # q = p = 1 there, 0 elsewhere
+        x[0] = -math.inf
+        loss, lse = ops.distill(x, ids, t)
+        assert loss[0].isnan() and lse[0] == -math.inf and loss[1] == 0
+
+
 def test_id_past_the_vocabulary_gives_nan():
     from kvstreams import ops
 

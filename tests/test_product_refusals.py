@@ -41,7 +41,7 @@ def _grads(**kw):
     (dict(weight_up=P, ld_w_up=64, residual=P, ld_res=32), E_ARG),
     (dict(weight_up=P, ld_w_up=64, pre=P, ld_pre=63), E_ARG),
     (dict(dtype=0), E_UNSUPPORTED), (dict(dtype=1), E_UNSUPPORTED), (dict(dtype=9), E_UNSUPPORTED),
-    (dict(k=60), E_UNSUPPORTED), (dict(ld_x=68), E_UNSUPPORTED), (dict(ld_w=68), E_UNSUPPORTED),
+    (dict(k=60), E_UNSUPPORTED), (dict(rows=(1 << 30) + 1), E_UNSUPPORTED), (dict(ld_x=68), E_UNSUPPORTED), (dict(ld_w=68), E_UNSUPPORTED),
     (dict(x=P + 2), E_UNSUPPORTED), (dict(weight=P + 8), E_UNSUPPORTED),
     (dict(weight_up=P + 8, ld_w_up=64), E_UNSUPPORTED), (dict(pre=P, ld_pre=32, pre_dtype=3), E_UNSUPPORTED),
 ])
