@@ -1161,12 +1161,24 @@ template <typename K> int max_pairs(K kernel, KernelState& s) {
 // 0.29 for 256 columns, which the tensor cores bound, but 0.235 for 128, which the 64 bytes per clock
 // that an SM takes from L2 bound (24 KB a block against 32).  Cut units cost about 6 (19 MB of sums
 // written at once) and 3 for each pair whose sums the last one to finish has to add.
+//
+// Pairs with cut units are at different K blocks, so they share operands only through L2: units are
+// cut where the operands of the cut ones come to at most 200 MB, and where that gains four percent.
+// Weight gradients (k_in x n_out from so many rows), whole tiles against cut: 4096 x 4096 from 8192
+// rows 239 -> 220 us, from 16384 532 -> 439; 6144 x 4096 from 16384 782 -> 674; but 4096 x 4096 from
+// 32768 (386 MB) 971 -> 1065, and an input gradient of 8192 x 4096 over 28672 (367 MB) 1885 -> 2050.
 constexpr int PAIRS = 74;  // of a B200's 148 SMs
 struct PairPlan {
   int bn, whole, cut_pairs;
   double us;
   size_t scratch() const { return (size_t)cut_pairs * 2 * EPI_WARPS * (SUMS_PER_WARP * 4 + 8); }
 };
+// A group of row blocks passes over all of B once: where B is too large to stay in L2 (126 MB, shared
+// with A and the results), fewer passes of it are worth more rows of A in flight.  8192 x 14336
+// gated x 4096: 1345 us in groups of 16, 1390 of 8; with B of 34 MB 215 us of 8, 218 of 16.
+int group_of(int64_t N, int kb, bool gated) {
+  return 2 * N * (gated ? 2 : 1) * kb * BK > (48 << 20) ? 16 : 8;
+}
 PairPlan pair_plan(int64_t row_blocks, int64_t N, int kb, bool gated, bool cut_allowed) {
   auto units_of = [&](int bn) { return row_blocks * ((N + (gated ? bn / 2 : bn) - 1) / (gated ? bn / 2 : bn)); };
   auto rounds = [](int64_t units) { return (double)((units + PAIRS - 1) / PAIRS); };
@@ -1176,12 +1188,17 @@ PairPlan pair_plan(int64_t row_blocks, int64_t N, int kb, bool gated, bool cut_a
   if (narrow < best.us) best = {128, (int)std::min<int64_t>(units_of(128), 1 << 30), 0, narrow};
   if (!cut_allowed || units % PAIRS == 0 || units >= (1 << 30)) return best;
   const int64_t whole = std::max<int64_t>(0, units / PAIRS - 1) * PAIRS, rest = units - whole;
+  const int64_t cols = units / row_blocks;
+  const int64_t r = std::max(std::min<int64_t>(row_blocks, group_of(N, kb, gated)), (rest + cols - 1) / cols);
+  const int64_t c = std::min(cols, (rest + r - 1) / r);
+  if ((r + c) * 256 * kb * BK * 2 > (int64_t)200 << 20) return best;
+  const double uncut = best.us;
   auto consider = [&](int64_t pairs, int others) {
     const double run = (double)rest * kb / pairs;  // K blocks a pair
     if (run < 4) return;
     const double us = 6.0 + (double)(whole / PAIRS) * (1.5 + kb * 0.29) + run * 0.29 + 1.5 * (1 + (run > kb)) +
                       6.0 + 3.0 * others;
-    if (us < best.us) best = {256, (int)whole, (int)pairs, us};
+    if (us < best.us && us < 0.96 * uncut) best = {256, (int)whole, (int)pairs, us};
   };
   // equal cuts of every unit, or all pairs whatever the cuts come to
   for (int s = 2; rest < PAIRS && rest * s <= PAIRS; ++s) consider(rest * s, s - 1);
@@ -1242,11 +1259,7 @@ int launch_pair_n(const Product& g, const PairPlan& plan, int32_t dtype, cudaStr
   if (units > (1 << 30)) return KVS_E_UNSUPPORTED;
   p.n_units = p.whole = (int)units;
   p.cut_pairs = 0;
-  // A group of row blocks passes over all of B once: where B is too large to stay in L2 (126 MB, shared
-  // with A and the results), fewer passes of it are worth more rows of A in flight.  8192 x 14336
-  // gated x 4096: 1345 us in groups of 16, 1390 of 8; with B of 34 MB 215 us of 8, 218 of 16.
-  const int64_t b_bytes = 2 * (int64_t)p.N * (GATED ? 2 : 1) * p.n_kb * p.k_parts * BK;
-  p.group = b_bytes > (48 << 20) ? 16 : 8;
+  p.group = group_of(p.N, p.n_kb * p.k_parts, GATED);
   int pairs = std::min(most, p.n_units);
   if (BN == 256 && plan.cut_pairs > 0 && most >= PAIRS) {
     p.whole = plan.whole;
