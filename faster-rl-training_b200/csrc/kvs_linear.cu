@@ -1162,11 +1162,13 @@ template <typename K> int max_pairs(K kernel, KernelState& s) {
 // that an SM takes from L2 bound (24 KB a block against 32).  Cut units cost about 6 (19 MB of sums
 // written at once) and 3 for each pair whose sums the last one to finish has to add.
 //
-// Pairs with cut units are at different K blocks, so they share operands only through L2: units are
-// cut where the operands of the cut ones come to at most 200 MB, and where that gains four percent.
-// Weight gradients (k_in x n_out from so many rows), whole tiles against cut: 4096 x 4096 from 8192
-// rows 239 -> 220 us, from 16384 532 -> 439; 6144 x 4096 from 16384 782 -> 674; but 4096 x 4096 from
-// 32768 (386 MB) 971 -> 1065, and an input gradient of 8192 x 4096 over 28672 (367 MB) 1885 -> 2050.
+// Pairs with cut units are at different K blocks and share operands only through L2, of which about
+// 90 MB holds them (110 where both operands lie MN-major: a K block of all tiles is then contiguous):
+// what does not fit comes from HBM again for every pair, 64 KB a K block.  Units are cut where the
+// larger of the two times gains four percent.  Weight gradients, whole tiles against cut: 4096 x 4096
+// from 8192 rows 239 -> 220 us, from 16384 532 -> 439, 6144 x 4096 from 16384 782 -> 674; forward
+// 4000 x 2560 x 8192 172 -> 138.  Not cut: a 4096 x 4096 weight gradient from 32768 rows (971 us,
+// cut 1065), 2048 x 4096 x 14336 (165, cut 231), 8192 x 4096 over 28672 (1885, cut 2050).
 constexpr int PAIRS = 74;  // of a B200's 148 SMs
 struct PairPlan {
   int bn, whole, cut_pairs;
@@ -1175,11 +1177,13 @@ struct PairPlan {
 };
 // A group of row blocks passes over all of B once: where B is too large to stay in L2 (126 MB, shared
 // with A and the results), fewer passes of it are worth more rows of A in flight.  8192 x 14336
-// gated x 4096: 1345 us in groups of 16, 1390 of 8; with B of 34 MB 215 us of 8, 218 of 16.
+// gated x 4096: 1345 us in groups of 16, 1390 of 8; with B of 34 MB 215 us of 8, 218 of 16; and where
+// 16 row blocks do not stay in L2 themselves, 16384 x 4096 x 14336 takes 1513 in groups of 8, 1548 of 16.
 int group_of(int64_t N, int kb, bool gated) {
-  return 2 * N * (gated ? 2 : 1) * kb * BK > (48 << 20) ? 16 : 8;
+  const int64_t row = 2 * (int64_t)kb * BK;  // bytes
+  return N * (gated ? 2 : 1) * row > (48 << 20) && 16 * 256 * row <= (48 << 20) ? 16 : 8;
 }
-PairPlan pair_plan(int64_t row_blocks, int64_t N, int kb, bool gated, bool cut_allowed) {
+PairPlan pair_plan(int64_t row_blocks, int64_t N, int kb, bool gated, bool both_mn, bool cut_allowed) {
   auto units_of = [&](int bn) { return row_blocks * ((N + (gated ? bn / 2 : bn) - 1) / (gated ? bn / 2 : bn)); };
   auto rounds = [](int64_t units) { return (double)((units + PAIRS - 1) / PAIRS); };
   const int64_t units = units_of(256);
@@ -1191,22 +1195,25 @@ PairPlan pair_plan(int64_t row_blocks, int64_t N, int kb, bool gated, bool cut_a
   const int64_t cols = units / row_blocks;
   const int64_t r = std::max(std::min<int64_t>(row_blocks, group_of(N, kb, gated)), (rest + cols - 1) / cols);
   const int64_t c = std::min(cols, (rest + r - 1) / r);
-  if ((r + c) * 256 * kb * BK * 2 > (int64_t)200 << 20) return best;
+  const double shared_mb = (double)(r + c) * 256 * kb * BK * 2 / 1e6, fits_mb = both_mn ? 110.0 : 90.0;
+  if (shared_mb > 250.0) return best;
+  const double hbm_us = shared_mb > fits_mb ? (double)rest * kb * 65536.0 * (1.0 - fits_mb / shared_mb) / 6.4e6 : 0.0;
   const double uncut = best.us;
-  auto consider = [&](int64_t pairs, int others) {
+  auto consider = [&](int64_t pairs, int others, bool in_step) {
     const double run = (double)rest * kb / pairs;  // K blocks a pair
     if (run < 4) return;
-    const double us = 6.0 + (double)(whole / PAIRS) * (1.5 + kb * 0.29) + run * 0.29 + 1.5 * (1 + (run > kb)) +
-                      6.0 + 3.0 * others;
+    const double us = 6.0 + (double)(whole / PAIRS) * (1.5 + kb * 0.29) + std::max(run * 0.29, in_step ? 0.0 : hbm_us) +
+                      1.5 * (1 + (run > kb)) + 6.0 + 3.0 * others;
     if (us < best.us && us < 0.96 * uncut) best = {256, (int)whole, (int)pairs, us};
   };
-  // equal cuts of every unit, or all pairs whatever the cuts come to
-  for (int s = 2; rest < PAIRS && rest * s <= PAIRS; ++s) consider(rest * s, s - 1);
-  consider(PAIRS, rest >= PAIRS ? 1 : (int)((PAIRS + rest - 1) / rest));
+  // equal cuts of every unit (pairs with the same part of theirs keep in step), or all pairs whatever
+  // the cuts come to
+  for (int s = 2; rest < PAIRS && rest * s <= PAIRS; ++s) consider(rest * s, s - 1, true);
+  consider(PAIRS, rest >= PAIRS ? 1 : (int)((PAIRS + rest - 1) / rest), false);
   return best;
 }
-PairPlan pair_plan_of(int64_t M, int m_parts, int64_t N, int kb, bool gated, bool cut_allowed) {
-  return pair_plan((M + 2 * BM - 1) / (2 * BM) * m_parts, N, kb, gated, cut_allowed);
+PairPlan pair_plan_of(int64_t M, int m_parts, int64_t N, int kb, bool gated, bool both_mn, bool cut_allowed) {
+  return pair_plan((M + 2 * BM - 1) / (2 * BM) * m_parts, N, kb, gated, both_mn, cut_allowed);
 }
 
 struct Product {
@@ -1348,9 +1355,9 @@ int launch_stream(const Operand (&w)[2], const Operand (&x)[2], StreamParams p, 
 
 template <typename T, bool A_MN, bool B_MN, int EPI>
 int launch_pair(const Product& g, int32_t dtype, cudaStream_t st) {
-  PairPlan plan = pair_plan_of(g.p.M, g.p.m_parts, g.p.N, g.p.n_kb * g.p.k_parts, EPI == EPI_GATED, true);
+  PairPlan plan = pair_plan_of(g.p.M, g.p.m_parts, g.p.N, g.p.n_kb * g.p.k_parts, EPI == EPI_GATED, A_MN && B_MN, true);
   if (plan.scratch() > g.scratch_bytes)
-    plan = pair_plan_of(g.p.M, g.p.m_parts, g.p.N, g.p.n_kb * g.p.k_parts, EPI == EPI_GATED, false);
+    plan = pair_plan_of(g.p.M, g.p.m_parts, g.p.N, g.p.n_kb * g.p.k_parts, EPI == EPI_GATED, A_MN && B_MN, false);
   return plan.bn == 128 ? launch_pair_n<T, A_MN, B_MN, EPI, 128>(g, plan, dtype, st)
                         : launch_pair_n<T, A_MN, B_MN, EPI, 256>(g, plan, dtype, st);
 }
@@ -1365,13 +1372,14 @@ bool use_stream(int64_t M, int64_t N, int kb_all, bool gated) {
   const int64_t ctas = ((N + (gated ? 63 : 127)) / (gated ? 64 : 128)) * ((M + s.tn - 1) / s.tn) * s.split;
   const double per_sm = (double)((ctas + 147) / 148);
   const double us = 6.5 + per_sm * ((kb_all + s.split - 1) / s.split * (TILE_BYTES + s.tn * BK * 2) / 115e3 + s.tn * 0.02);
-  return us < pair_plan_of(M, 1, N, kb_all, gated, true).us;
+  return us < pair_plan_of(M, 1, N, kb_all, gated, false, true).us;
 }
 
 // scratch of one product for its cut units (0: none)
-size_t product_scratch(int64_t M, int m_parts, int64_t N, int kb_all, bool gated, bool may_stream) {
-  if (may_stream && use_stream(M, N, kb_all, gated)) return 0;
-  return pair_plan_of(M, m_parts, N, kb_all, gated, true).scratch();
+// (a weight gradient's operands both lie MN-major, and it has no few-rows form)
+size_t product_scratch(int64_t M, int m_parts, int64_t N, int kb_all, bool gated, bool weight_grad) {
+  if (!weight_grad && use_stream(M, N, kb_all, gated)) return 0;
+  return pair_plan_of(M, m_parts, N, kb_all, gated, weight_grad, true).scratch();
 }
 
 bool act_ok(int32_t a) { return a >= KVS_ACT_NONE && a <= KVS_ACT_GELU; }
@@ -1454,8 +1462,8 @@ int dx_blocks(const kvs_linear_args* a) { return (a->n + BK - 1) / BK * (a->weig
 int dw_blocks(const kvs_linear_args* a) { return (a->rows + BK - 1) / BK; }
 // scratch of the larger of the two (they run one after the other)
 size_t backward_product_scratch(const kvs_linear_args* a, const kvs_linear_grads* g) {
-  const size_t x = g->dx ? product_scratch(a->rows, 1, a->k, dx_blocks(a), false, true) : 0;
-  const size_t w = g->dw ? product_scratch(a->n, a->weight_up ? 2 : 1, a->k, dw_blocks(a), false, false) : 0;
+  const size_t x = g->dx ? product_scratch(a->rows, 1, a->k, dx_blocks(a), false, false) : 0;
+  const size_t w = g->dw ? product_scratch(a->n, a->weight_up ? 2 : 1, a->k, dw_blocks(a), false, true) : 0;
   return std::max(x, w);
 }
 // what lies before it: dz and the bias partials
@@ -1566,7 +1574,7 @@ template <typename T, typename Z> int backward(const kvs_linear_args* a, const k
 
 KVS_API size_t kvs_linear_scratch_bytes(const kvs_linear_args* a) {
   if (!a || a->rows <= 0 || a->n <= 0 || a->k <= 0) return 0;
-  return product_scratch(a->rows, 1, a->n, (a->k + BK - 1) / BK, a->weight_up != nullptr, true);
+  return product_scratch(a->rows, 1, a->n, (a->k + BK - 1) / BK, a->weight_up != nullptr, false);
 }
 
 KVS_API int kvs_linear(const kvs_linear_args* a, kvs_stream_t stream) {
