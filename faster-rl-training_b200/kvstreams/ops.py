@@ -706,21 +706,27 @@ def gated_linear_backward(gh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tenso
 def _distill_args(logits, ids, teacher):
     if not (logits.is_cuda and ids.is_cuda and teacher.is_cuda):
         _check_cuda(logits, ids, teacher)
-    if logits.dtype not in N.DTYPE_CODE:
+    code = N.DTYPE_CODE.get(logits.dtype)
+    if code is None:
         raise ValueError(f"unsupported logits dtype {logits.dtype}")
     if logits.dim() != 2 or logits.shape[1] == 0 or logits.stride(1) != 1:
         raise ValueError("logits must be a 2-D tensor with contiguous rows")
-    if ids.dim() != 2 or ids.shape[0] != logits.shape[0] or ids.shape[1] == 0 or tuple(teacher.shape) != tuple(ids.shape):
-        raise ValueError(f"ids and teacher must be [{logits.shape[0]}, top] "
-                         f"(got {tuple(ids.shape)} and {tuple(teacher.shape)})")
-    if ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
-        raise ValueError(f"ids must be integers (got {ids.dtype})")
+    n, vocab = logits.shape
+    if ids.dim() != 2 or ids.shape[0] != n or ids.shape[1] == 0 or teacher.shape != ids.shape:
+        raise ValueError(f"ids and teacher must be [{n}, top] (got {tuple(ids.shape)} and {tuple(teacher.shape)})")
     if ids.device != logits.device or teacher.device != logits.device:
         raise ValueError("logits, ids and teacher must be on one device")
-    acc = torch.float64 if logits.dtype == torch.float64 else torch.float32
-    if logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]:  # an expanded row
-        logits = logits.contiguous()
-    return logits, ids.to(torch.long).contiguous(), teacher.to(acc).contiguous(), acc
+    acc = torch.float64 if code == N.KVS_F64 else torch.float32
+    if ids.dtype is not torch.long:
+        if ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
+            raise ValueError(f"ids must be integers (got {ids.dtype})")
+        ids = ids.to(torch.long)
+    if teacher.dtype is not acc:
+        teacher = teacher.to(acc)
+    ld = logits.stride(0) if n > 1 else vocab
+    if ld < vocab:  # an expanded row
+        logits, ld = logits.contiguous(), vocab
+    return logits, ids.contiguous(), teacher.contiguous(), acc, code, ld
 
 
 def distill(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, temperature: float = 1.0):
@@ -732,13 +738,12 @@ def distill(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, temp
 
     A slot with a negative id, or a teacher value of -inf or NaN, is empty; a row without kept
     slots has loss 0.  One pass over each row; float32 results (float64 for float64 logits)."""
-    logits, i, t, acc = _distill_args(logits, ids, teacher)
+    logits, i, t, acc, code, ld = _distill_args(logits, ids, teacher)
     n, vocab = logits.shape
     loss = logits.new_empty((n,), dtype=acc)
-    lse = logits.new_empty((n,), dtype=acc)
-    _launch(logits, N.launch_lib().kvs_distill, "kvs_distill", logits.data_ptr(), _pitch(logits), n, vocab,
-            i.data_ptr(), t.data_ptr(), i.shape[1], temperature, N.DTYPE_CODE[logits.dtype], loss.data_ptr(),
-            lse.data_ptr())
+    lse = torch.empty_like(loss)
+    _launch(logits, N.launch_lib().kvs_distill, "kvs_distill", logits.data_ptr(), ld, n, vocab, i.data_ptr(),
+            t.data_ptr(), i.shape[1], temperature, code, loss.data_ptr(), lse.data_ptr())
     return loss, lse
 
 
@@ -749,29 +754,25 @@ def distill_backward(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Ten
     and the forward's ``lse``, in ``out_dtype`` (the logits' type; bf16 / fp16 from float32 logits).
     ``out`` may be ``logits`` itself.  Rows without kept slots get zeros."""
     given = logits
-    logits, i, t, acc = _distill_args(logits, ids, teacher)
+    logits, i, t, acc, code, ld = _distill_args(logits, ids, teacher)
     n, vocab = logits.shape
     for name, v in (("lse", lse), ("grad", grad)):
-        if tuple(v.shape) != (n,) or v.device != logits.device:
+        if v.shape != (n,) or v.device != logits.device:
             raise ValueError(f"{name} must be [{n}] on {logits.device}")
     l, g = lse.to(acc).contiguous(), grad.to(acc).contiguous()
     if out is None:
         out = logits.new_empty((n, vocab), dtype=out_dtype or logits.dtype)
+    elif out is not given and _overlap(out, logits):
+        raise ValueError("out may be the logits tensor itself, but not overlap it otherwise")
     elif (tuple(out.shape) != (n, vocab) or out.device != logits.device or out.dtype != (out_dtype or out.dtype)
           or (vocab > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < vocab)):
         raise ValueError(f"out must be [{n}, {vocab}] with dense rows on {logits.device}, of type {out_dtype}")
-    if out is not given and _overlap(out, logits):
-        raise ValueError("out may be the logits tensor itself, but not overlap it otherwise")
     if out.dtype not in N.DTYPE_CODE:
         raise ValueError(f"unsupported gradient dtype {out.dtype}")
-    _launch(logits, N.launch_lib().kvs_distill_backward, "kvs_distill_backward", logits.data_ptr(), _pitch(logits), n,
-            vocab, i.data_ptr(), t.data_ptr(), i.shape[1], l.data_ptr(), g.data_ptr(), temperature,
-            N.DTYPE_CODE[logits.dtype], out.data_ptr(), _pitch(out), N.DTYPE_CODE[out.dtype])
+    _launch(logits, N.launch_lib().kvs_distill_backward, "kvs_distill_backward", logits.data_ptr(), ld, n, vocab,
+            i.data_ptr(), t.data_ptr(), i.shape[1], l.data_ptr(), g.data_ptr(), temperature, code, out.data_ptr(),
+            out.stride(0) if n > 1 else vocab, N.DTYPE_CODE[out.dtype])
     return out
-
-
-def _pitch(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _span(t: torch.Tensor):

@@ -83,6 +83,15 @@ def test_backward_scratch(lib):
     assert size(dict(rows=0), dict(db=P)) == 0
 
 
+def test_forward_scratch(lib):
+    """Only products whose tiles do not come out even have scratch to gain from, and few rows never."""
+    size = lambda **kw: lib.kvs_linear_scratch_bytes(C.byref(_args(**kw)))  # noqa: E731
+    assert lib.kvs_linear_scratch_bytes(None) == 0
+    assert size() == 0 and size(rows=0) == 0
+    assert size(rows=128, n=4096, k=14336, ld_x=14336, ld_w=14336, ld_out=4096) == 0
+    assert size(rows=1536, n=4096, k=4096, ld_x=4096, ld_w=4096, ld_out=4096) > 0
+
+
 def _distill(lib, **kw):
     a = {**dict(logits=P, ld=100, n_rows=2, vocab=100, ids=P, teacher=P, top=4, temperature=1.0, dtype=0, loss=P,
                 lse=P), **kw}
