@@ -186,6 +186,80 @@ def test_two_streams_and_threads():
     assert not bad
 
 
+CUT = (600, 1500, 14344)  # rows, n, k of a product whose tiles are cut among the pairs of CTAs
+
+
+def test_cut_product_captured_and_replayed():
+    """A cut product's flags are left clean: replays of two graphs in turn, with eager calls between,
+    equal the eager results, and a row with a NaN stays alone."""
+    from kvstreams import ops
+
+    rows, n, k = CUT
+    w, u = _rand(2, n, k, scale=0.05), _rand(3, n, k, scale=0.05)
+    graphs = []
+    for seed in (1, 2):
+        x = _rand(10 + seed, rows, k)
+        ops.linear(x, w)
+        ops.gated_linear(x, w, u)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = ops.linear(x, w, activation="silu")
+            h = ops.gated_linear(x, w, u)
+        graphs.append((g, x, y, h))
+    for round_ in range(4):
+        for i, (g, x, y, h) in enumerate(graphs):
+            x.copy_(_rand(100 + 10 * round_ + i, rows, k))
+            if round_ == 3:
+                x[7, 3] = math.nan
+        for g, *_ in graphs:
+            g.replay()
+        for g, x, y, h in graphs:
+            assert torch.equal(y.nan_to_num(), ops.linear(x, w, activation="silu").nan_to_num())
+            assert torch.equal(h.nan_to_num(), ops.gated_linear(x, w, u).nan_to_num())
+            bad = y.isnan().any(1)
+            assert bad.sum().item() == (1 if round_ == 3 else 0) and (round_ < 3 or y[7].isnan().all())
+
+
+def test_cut_products_on_two_streams():
+    from kvstreams import ops
+
+    rows, n, k = CUT
+    xs = [_rand(s, rows, k) for s in (1, 2)]
+    ws = [_rand(s + 5, n, k, scale=0.05) for s in (1, 2)]
+    want = [ops.linear(x, w) for x, w in zip(xs, ws)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.linear(xs[i], ws[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def test_long_rows_captured():
+    """Few long logits rows (a cluster per row) in a graph."""
+    from kvstreams import ops
+
+    x = _rand(1, 3, 50000, dtype=torch.float32)
+    ids, t, g1 = torch.randint(0, 50000, (3, 9), device="cuda"), _rand(2, 3, 9, dtype=torch.float32), torch.rand(3, device="cuda")
+    ops.distill_backward(x, ids, t, ops.distill(x, ids, t)[1], g1)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        loss, lse = ops.distill(x, ids, t)
+        d = ops.distill_backward(x, ids, t, lse, g1)
+    for seed in (3, 4):
+        x.copy_(_rand(seed, 3, 50000, dtype=torch.float32))
+        g.replay()
+        l2, e2 = ops.distill(x, ids, t)
+        assert torch.equal(loss, l2) and torch.equal(lse, e2)
+        assert torch.equal(d, ops.distill_backward(x, ids, t, e2, g1))
+
+
 def test_offsets_past_32_bits():
     """Results of more than 2^31 elements: the last rows and columns are where they belong."""
     from kvstreams import ops
