@@ -737,7 +737,8 @@ def distill(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, temp
         loss = sum_j p_j (log p_j - log_softmax(logits / T)[ids_j]),   lse = logsumexp(logits / T)
 
     A slot with a negative id, or a teacher value of -inf or NaN, is empty; a row without kept
-    slots has loss 0.  One pass over each row; float32 results (float64 for float64 logits)."""
+    slots has loss 0; a row with an id past the vocabulary has loss NaN.  At most 1024 slots a row.
+    One pass over each row; float32 results (float64 for float64 logits)."""
     logits, i, t, acc, code, ld = _distill_args(logits, ids, teacher)
     n, vocab = logits.shape
     loss = logits.new_empty((n,), dtype=acc)

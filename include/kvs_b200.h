@@ -495,8 +495,8 @@ int kvs_silu_mul_backward(const void* gu, const void* grad, void* dgu, int64_t n
  * rows are ld_* elements apart.  pre (optional) receives the pre-activations for the backward:
  * [rows][n], or [rows][2 n] = gate | up, in pre_dtype (KVS_F32, or dtype: half the memory, one more
  * rounding in the gradients).  out may be the residual.
- * Any rows (0: nothing happens; at most 2^30) and n; k and the pitches of x and the weights multiples
- * of 8, their bases 16-byte aligned (KVS_E_UNSUPPORTED otherwise).  A bounded wait inside a kernel that runs
+ * Any rows (0: nothing happens; at most 2^30) and n (at most 2^29); k (at most 2^30) and the pitches of
+ * x and the weights multiples of 8, their bases 16-byte aligned (KVS_E_UNSUPPORTED otherwise).  A bounded wait inside a kernel that runs
  * out gives NaN outputs. */
 enum kvs_activation { KVS_ACT_NONE = 0, KVS_ACT_RELU = 1, KVS_ACT_SILU = 2, KVS_ACT_GELU = 3 /* erf form */ };
 typedef struct kvs_linear_args {

@@ -92,6 +92,15 @@ def test_forward_scratch(lib):
     assert size(rows=1536, n=4096, k=4096, ld_x=4096, ld_w=4096, ld_out=4096) > 0
 
 
+def test_scratch_of_sizes_past_the_limits(lib):
+    """Sizes that the calls refuse have no scratch, also where their block counts would pass 32 bits."""
+    for kw in (dict(k=2**31 - 8), dict(n=2**31 - 1), dict(n=(1 << 29) + 8), dict(rows=2**31 - 1)):
+        a = _args(**{**dict(rows=300), **kw})
+        assert lib.kvs_linear_scratch_bytes(C.byref(a)) == 0
+        assert lib.kvs_linear_backward_scratch_bytes(C.byref(a), C.byref(_grads(db=P))) == 0
+        assert lib.kvs_linear(C.byref(a), None) == E_UNSUPPORTED
+
+
 def _distill(lib, **kw):
     a = {**dict(logits=P, ld=100, n_rows=2, vocab=100, ids=P, teacher=P, top=4, temperature=1.0, dtype=0, loss=P,
                 lse=P), **kw}
