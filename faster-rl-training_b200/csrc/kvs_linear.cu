@@ -47,6 +47,7 @@
 #include <algorithm>
 #include <atomic>
 #include <chrono>
+#include <cmath>
 #include <mutex>
 #include <type_traits>
 
@@ -727,6 +728,26 @@ struct StreamParams {
   int64_t ld_out, ld_res, ld_pre;
 };
 
+// A walk round a ring of stages: the stage at hand and the parity of its barriers' phase.  (Counted
+// on, not divided out of a running index: the one thread that issues copies, or MMAs, does nothing else,
+// and at 16 rows of x its instructions, not the copies, bounded a K block.)
+struct Ring {
+  uint32_t slot = 0, phase = 0;
+  __device__ __forceinline__ void next(uint32_t stages) {
+    if (++slot == stages) {
+      slot = 0;
+      phase ^= 1;
+      wrapped = true;
+    }
+  }
+  // whether stage j was filled, and the parity of its last fill's phase
+  __device__ __forceinline__ bool used(uint32_t j) const { return wrapped || j < slot; }
+  __device__ __forceinline__ uint32_t last_phase(uint32_t j) const { return j < slot ? phase : phase ^ 1; }
+
+ private:
+  bool wrapped = false;
+};
+
 template <typename T, bool W_MN, bool GATED>
 __global__ void __launch_bounds__(SNT)
 stream_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant__ CUtensorMap tm_w1,
@@ -769,10 +790,10 @@ stream_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_const
   if (warp == 0) {
     if (lane == 0) {
       bool ok = true;
-      int it = 0;
-      for (int k = kb_beg; k < kb_end; ++k, ++it) {
-        const int s = it % p.stages;
-        if (it >= p.stages && !mbar_wait_fast(&empty[s], ((it / p.stages) - 1) & 1, abort_flag)) {
+      Ring at;
+      for (int k = kb_beg; k < kb_end; ++k, at.next(p.stages)) {
+        const int s = at.slot;
+        if (!mbar_wait_fast(&empty[s], at.phase ^ 1, abort_flag)) {  // (true the first time round)
           ok = false;
           break;
         }
@@ -794,24 +815,23 @@ stream_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_const
       }
       if (!ok) *abort_flag = 1;
       // every copy has landed before the CTA may go on to leave; immediate unless aborting
-      for (int j = max(0, it - p.stages); j < it; ++j)
-        mbar_wait(&full[j % p.stages], (j / p.stages) & 1, nullptr, ok ? 400000 : 20000);
+      for (int j = 0; j < p.stages; ++j)
+        if (at.used(j)) mbar_wait(&full[j], at.last_phase(j), nullptr, ok ? 400000 : 20000);
       mbar_arrive(drained);
     }
   } else if (warp == 1) {
     const uint32_t idesc = idesc_of<T>(128, p.tn, W_MN, 0);
     constexpr uint32_t AS = W_MN ? 128 : 2;
-    const uint32_t base = smem_addr(smem);
+    const uint64_t dw0 = operand_desc<W_MN>(smem_addr(smem)), dx0 = desc_kmajor_sw128(smem_addr(smem) + TILE_BYTES);
     bool ok = true;
-    int it = 0;
-    for (int k = kb_beg; k < kb_end; ++k, ++it) {
-      const int s = it % p.stages;
-      ok = __all_sync(0xffffffffu, mbar_wait_fast(&full[s], (it / p.stages) & 1, abort_flag));
+    Ring at;
+    for (int k = kb_beg; k < kb_end; ++k, at.next(p.stages)) {
+      const int s = at.slot;
+      ok = __all_sync(0xffffffffu, mbar_wait_fast(&full[s], at.phase, abort_flag));
       if (!ok) break;
       tc_fence_after();
-      const uint32_t at = base + s * stage_bytes;
-      const uint64_t dw = operand_desc<W_MN>(at), dx = desc_kmajor_sw128(at + TILE_BYTES);
-      umma_bf16_warp_at<0, 0>(tmem, dw, dx, idesc, it > 0);
+      const uint64_t dw = dw0 + s * (stage_bytes >> 4), dx = dx0 + s * (stage_bytes >> 4);
+      umma_bf16_warp_at<0, 0>(tmem, dw, dx, idesc, k > kb_beg);
       umma_bf16_warp_at<AS, 2>(tmem, dw, dx, idesc, 1);
       umma_bf16_warp_at<2 * AS, 4>(tmem, dw, dx, idesc, 1);
       umma_bf16_warp_at<3 * AS, 6>(tmem, dw, dx, idesc, 1);
@@ -1199,8 +1219,8 @@ template <typename K> int max_pairs(K kernel, KernelState& s) {
 // K blocks of the others, and the estimate in microseconds by which the cut was chosen (B200,
 // measured at 512..8192 x 4096 x 4096).  About 6 outside the loop, 1.5 a unit, and per K block
 // 0.29 for 256 columns, which the tensor cores bound, but 0.235 for 128, which the 64 bytes per clock
-// that an SM takes from L2 bound (24 KB a block against 32).  Cut units cost about 6 (19 MB of sums
-// written at once) and 3 for each pair whose sums the last one to finish has to add.
+// that an SM takes from L2 bound (24 KB a block against 32).  Cut units cost about 7 (19 MB of sums
+// written at once; less with fewer pairs) and 2 for each pair whose sums the last one to finish has to add.
 //
 // Pairs with cut units are at different K blocks and share operands only through L2, of which about
 // 90 MB holds them (110 where both operands lie MN-major: a K block of all tiles is then contiguous):
@@ -1243,7 +1263,7 @@ PairPlan pair_plan(int64_t row_blocks, int64_t N, int kb, bool gated, bool both_
     const double run = (double)rest * kb / pairs;  // K blocks a pair
     if (run < 4) return;
     const double us = 6.0 + (double)(whole / PAIRS) * (1.5 + kb * 0.29) + std::max(run * 0.29, in_step ? 0.0 : hbm_us) +
-                      1.5 * (1 + (run > kb)) + 6.0 + 3.0 * others;
+                      1.5 * (1 + (run > kb)) + 7.0 * (double)pairs / PAIRS + 2.0 * others;
     if (us < best.us && us < 0.96 * uncut) best = {256, (int)whole, (int)pairs, us};
   };
   // equal cuts of every unit (pairs with the same part of theirs keep in step), or all pairs whatever
@@ -1320,9 +1340,40 @@ int launch_pair_n(const Product& g, const PairPlan& plan, int32_t dtype, cudaStr
                            o[2], p);
 }
 
+// clusters of `size` (2, 4, 8) of the stream kernel's CTAs that run at once, one CTA an SM
+int clusters_at_once(int size) {
+  static int most[64][3];  // by device; 0: not asked yet
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();
+    return size == 2 ? 74 : size == 4 ? 33 : 15;  // planning without a device: a B200's
+  }
+  std::lock_guard<std::mutex> lock(g_mu);
+  int& n = most[dev][size / 4];
+  if (n == 0) {
+    const auto kernel = stream_gemm_kernel<__nv_bfloat16, false, false>;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(size, 1, 1);
+    cfg.blockDim = dim3(SNT, 1, 1);
+    cfg.dynamicSmemBytes = 200 * 1024;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = 1;
+    }
+  }
+  return n;
+}
+
 // ---- few rows: how a product is cut for the stream kernel
 struct StreamPlan {
-  int tn, stages, split;
+  int tn, stages, split, per_sm;
   size_t smem;
 };
 StreamPlan stream_plan(int64_t M, int64_t N, int kb_all, bool gated) {
@@ -1333,24 +1384,30 @@ StreamPlan stream_plan(int64_t M, int64_t N, int kb_all, bool gated) {
   const int stage = TILE_BYTES + s.tn * BK * 2;
   const int fixed = S_BAR_BYTES + 1024;
   const int64_t tiles = ((N + (gated ? 63 : 127)) / (gated ? 64 : 128)) * mt;
-  // (powers of two: clusters of other sizes pack badly into the GPCs; 1 x 6144 x 4096 took 18.6 us
-  // with six CTAs a tile, 13.4 us with four)
-  auto cut = [&](int per_sm) {
+  // As many CTAs a tile as run at once with the whole shared memory as their ring, but with two K blocks
+  // each, four where the partial sums are large (128 x 1024 x 1024: 6.6 us in fours, 7.4 in eights).  What
+  // does not run at once waits for a whole round: 64 x 4608 x 4096 takes 12.4 us in clusters of two, 18.0
+  // of four, and 2048 columns of K 4096 8.6 in fours, 14.5 in eights.  (Powers of two: clusters of other
+  // sizes pack badly into the GPCs; 1 x 6144 x 4096 took 18.6 us with six CTAs a tile, 13.4 with four.)
+  auto cut = [&](int per_sm, int least) {
     int split = 1;
-    while (split < SMAX_SPLIT && tiles * split * 2 <= per_sm * 148 && kb_all / (split * 2) >= 2) split *= 2;
+    while (split < SMAX_SPLIT && tiles <= (int64_t)per_sm * clusters_at_once(split * 2) && kb_all / (split * 2) >= least)
+      split *= 2;
     return split;
   };
-  // Two CTAs an SM keep every SM loading; one, with the whole shared memory as its ring, halves the
-  // partial sums that an SM exchanges.  One is better where one CTA a SM fills the machine by itself
-  // and there are enough rows for the exchange to count: 64 x 4096 x 4096 12.1 us against 13.1,
-  // 128 x 4096 x 14336 27.7 against 30.3; but 64 x 6144 x 4096 (96 CTAs) 16.8 against 15.7, and
-  // 1 x 4096 x 14336 22.7 against 22.0.
-  int per_sm = 2;
-  const int64_t alone = tiles * cut(1);
-  if (mt == 1 && s.tn >= 32 && alone <= 148 && alone >= 126) per_sm = 1;
-  const int room = (per_sm == 1 ? 232448 : HALF_SM_SMEM) - fixed;
+  // One CTA an SM has the deeper ring and exchanges half the partial sums: 64 x 1024 x 4096 7.2 us against
+  // 7.9 with two an SM, 128 x 2048 x 14336 18.7 against 21.8.  Two an SM are better
+  //   for one to 16 rows, where their number lets a tile be cut once more: 1 x 4608 x 4096 9.9 against 11.1,
+  //   1 x 4608 x 14336 25.5 against 30.3;
+  //   for up to 64 rows of K >= 2048, where whole tiles leave SMs idle: 32 x 10240 x 4096 18.2 against 19.4;
+  //   and where there are more tiles than SMs: 64 x 28672 x 4096 45.4 against 47.8.
+  const int least = s.tn > 32 ? 4 : 2;
+  const int one = cut(1, least), two = cut(2, least);
+  const bool spread = two > one && (s.tn <= 16 || (one == 1 && s.tn <= 64 && kb_all >= 32));
+  s.per_sm = spread || tiles > 148 ? 2 : 1;
+  const int room = (s.per_sm == 1 ? 232448 : HALF_SM_SMEM) - fixed;
   s.stages = std::min(room / stage, SMAX_STAGES);  // three at least, which hold the 512 tn bytes of partial sums
-  s.split = cut(per_sm);
+  s.split = s.per_sm == 2 ? two : one;
   s.smem = (size_t)s.stages * stage + fixed;
   return s;
 }
@@ -1400,16 +1457,23 @@ int launch_pair(const Product& g, int32_t dtype, cudaStream_t st) {
 }
 
 // Whether a product of M rows goes to the stream kernel.  Up to 128 rows the weights' bytes bound
-// it (128 x 14336 gated x 4096: 48.1 us against 57 in pair units; 64 x 4096 x 14336: 25.0 against
-// 62).  Beyond, the estimate of what its SMs take from L2 (115 GB/s each) plus finishing decides:
-// 256 x 4096 x 4096 takes 17.7 us here, 22.6 in pairs.
+// it (128 x 14336 gated x 4096: 48.1 us against 57 in pair units; 64 x 4096 x 14336: 22.9 against
+// 62).  Beyond, two estimates decide, fitted to both kernels' times over 144..1536 rows, 1024..14336
+// columns and K 520..14336, back to back.  Here a K block takes a CTA 0.27 us, an SM takes 147 KB
+// and all of them 18 MB a microsecond from L2; a row of a tile costs 0.021 us to finish, a doubling of
+// the cluster 0.27.  What pair_plan says of the pairs is its time alone: of its 6 us about 3 are
+// hidden in a row of calls.  300 x 6144 x 4096 takes 19.7 us here, 26.2 in pairs; 256 x 1024 x 1024
+// 7.2 against 7.4; 640 x 4096 x 2048 18.7 against 15.4.  The choice is within 24 % of the better
+// one everywhere in that range, within 1 % on average.
 bool use_stream(int64_t M, int64_t N, int kb_all, bool gated) {
   if (M <= 128) return true;
   const StreamPlan s = stream_plan(M, N, kb_all, gated);
   const int64_t ctas = ((N + (gated ? 63 : 127)) / (gated ? 64 : 128)) * ((M + s.tn - 1) / s.tn) * s.split;
-  const double per_sm = (double)((ctas + 147) / 148);
-  const double us = 6.5 + per_sm * ((kb_all + s.split - 1) / s.split * (TILE_BYTES + s.tn * BK * 2) / 115e3 + s.tn * 0.02);
-  return us < pair_plan_of(M, 1, N, kb_all, gated, false, true).us;
+  const double rounds = (double)((ctas + 148 * s.per_sm - 1) / (148 * s.per_sm)), on_an_sm = (double)((ctas + 147) / 148);
+  const double blocks = (kb_all + s.split - 1) / s.split, bytes = blocks * (TILE_BYTES + s.tn * BK * 2);
+  const double us = 3.0 + std::max({rounds * blocks * 0.27, on_an_sm * bytes / 147e3, (double)ctas * bytes / 18.1e6}) +
+                    rounds * s.tn * 0.021 + std::log2((double)s.split) * 0.27 + (rounds - 1) * 3.3;
+  return us < 3.1 + 1.065 * (pair_plan_of(M, 1, N, kb_all, gated, false, true).us - 6.0);
 }
 
 // scratch of one product for its cut units (0: none)
