@@ -690,8 +690,8 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
 // places: 128 weight rows (or, in dx, 128 columns of W) are the M = 128 rows of the MMA and a tile
 // of 16..128 rows of x its N columns, so the tensor cores' work follows the rows that exist and
 // TMEM lane = result column.  A cluster of S CTAs takes one tile and splits the reduced index
-// between them, so that (result tiles x S) CTAs stream the weights at once, two per SM while a
-// CTA's ring fits half of its shared memory; each holds about 100 KB of copies in flight.  The S
+// between them, so that (result tiles x S) CTAs stream the weights at once, one per SM or two, each with
+// about 200 or 100 KB of copies in flight (stream_plan has the rule and both sides' times).  The S
 // partial sums meet in distributed shared memory: CTA r adds up, in rank order, the 128 / S result
 // columns that it then finishes (bias, activation, gate product, residual) and stores.  Nothing
 // passes through global memory, no counters, no second launch, and the order of the sum is fixed.
@@ -701,9 +701,9 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
 // 256 threads: warp 0 lane 0 = TMA producer, warp 1 = TMEM allocation and MMA issuer, warps 4..7
 // take the accumulators to shared memory; all of them finish and store.
 //
-// Bound by HBM where the weights are large: 1 x 14336 gated x 4096 takes 42.0 us (235 MB, 5.6 TB/s, 87 %
-// of a copy's rate), 48 rows 44.0, 64 x 4096 x 14336 26.4 (117 MB, 4.4 TB/s); else by what lies beside
-// the stream, 6 us of launch, first loads and join: 1 x 4096 x 4096 10.3 us for 34 MB.
+// Bound by HBM where the weights are large: 1 x 14336 gated x 4096 takes 40.8 us (235 MB, 5.8 TB/s, 89 %
+// of a copy's rate), 48 rows 43.3, 64 x 4096 x 14336 22.9 in a graph (117 MB, 5.1 TB/s); else by what
+// lies beside the stream, 5 us of launch, first loads and join: 1 x 4096 x 4096 10 us for 34 MB.
 constexpr int SNT = 256;
 constexpr int SMAX_STAGES = 8;
 constexpr int SMAX_SPLIT = 8;
