@@ -190,3 +190,17 @@ def test_cut_tiles(rows, n, k):
     _near(gx, dg @ w.double() + du @ u.double(), e * (dg.abs() @ aw + du.abs() @ au) + 2.0 ** -10, BF, "gated dx")
     _near(g1, dg.t() @ x.double(), e * dg.abs().t() @ ax + 2.0 ** -10, BF, "dw gate")
     _near(g2, du.t() @ x.double(), e * du.abs().t() @ ax + 2.0 ** -10, BF, "dw up")
+
+
+@pytest.mark.parametrize("rows", [8, 600])
+def test_gelu_over_its_range(rows):
+    """x W^T with W the identity is exact, so the output is gelu itself rounded once.  The normal
+    distribution's F is off by 7.5e-8 (its formula) and by three roundings of 2^-24 (1.8e-7), times |z|;
+    fp16 rounds by 2^-11 relative, below its normal numbers by 2^-25."""
+    from kvstreams import ops
+
+    z = torch.linspace(-10, 10, rows * 512, device="cuda").to(torch.float16).view(rows, 512)
+    w = torch.eye(512, device="cuda", dtype=torch.float16)
+    want = F.gelu(z.double())
+    bound = want.abs() * 2.0**-11 + z.double().abs() * 2.6e-7 + 2.0**-25
+    assert ((ops.linear(z, w, activation="gelu").double() - want).abs() <= bound).all()
