@@ -191,7 +191,7 @@ struct PairParams {
   void* pre;
   int64_t ld_out, ld_res, ld_pre;
   float* sums;                // [cut_pairs][2 CTAs][8 warps][4 chunks][8][32 lanes][4]: parts' float32 sums
-  unsigned long long* ready;  // [cut_pairs][2][8]: `token` once the sums are there
+  unsigned long long* ready;  // [cut_pairs][2][8]: flag words (flag_give / flag_take) of those sums
   unsigned long long token;   // of this launch; never that of another
 };
 
@@ -504,7 +504,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
           if (lane == 0) {
             mbar_arrive_cluster(acce + ab * 8);
             __threadfence();
-            st_release_gpu(p.ready + slot, p.token);
+            flag_give(p.ready + slot, p.token);
           }
           continue;
         }
@@ -516,11 +516,10 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
         while (pair + others + 1 < p.cut_pairs && cut_begin(p, kb_all, pair + others + 1) < unit_end) ++others;
         bool there = true;
         if (lane == 0) {
-          for (int r = 1; there && r <= others; ++r) {
-            const unsigned long long* flag = p.ready + ((pair + r) * 2 + (int)rank) * EPI_WARPS + w;
-            there = false;
-            for (int n = 0; n < (1 << 21) && !there; ++n) there = ld_acquire_gpu(flag) == p.token;  // over a second
-          }
+          // over a second for the first; after one that ran out the others are only looked at, so that each
+          // flag is left as flag_take leaves it
+          for (int r = 1; r <= others; ++r)
+            there &= flag_take(p.ready + ((pair + r) * 2 + (int)rank) * EPI_WARPS + w, p.token, there ? 1 << 21 : 1);
         }
         if (!__all_sync(0xffffffffu, there)) dead = true;
       }
@@ -668,11 +667,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
       // this thread's TMEM reads are done: release the accumulator to the MMA warp
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive_cluster(acce + ab * 8);
-        // the flags are left as no launch's token, for a replay of this one
-        for (int r = 1; r <= others; ++r) p.ready[((pair + r) * 2 + (int)rank) * EPI_WARPS + w] = 0;
-      }
+      if (lane == 0) mbar_arrive_cluster(acce + ab * 8);
     }
     if (lane == 0) bulk_wait_read<0>();  // the boxes have left shared memory before the CTA does
     __syncwarp();
@@ -1290,7 +1285,7 @@ unsigned long long launch_token() {
   z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
   z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
   z ^= z >> 31;
-  return z ? z : 1;
+  return z && ~z ? z : 1;  // (0 is the word of a flag that is not set, ~0 that of one given up)
 }
 
 template <typename T, bool A_MN, bool B_MN, int EPI, int BN>
@@ -1720,4 +1715,25 @@ KVS_API int kvs_linear_backward(const kvs_linear_args* a, const kvs_linear_grads
   const bool f32 = a->pre_dtype == KVS_F32;
   if (a->dtype == KVS_F16) return f32 ? backward<__half, float>(a, g, st) : backward<__half, __half>(a, g, st);
   return f32 ? backward<__nv_bfloat16, float>(a, g, st) : backward<__nv_bfloat16, __nv_bfloat16>(a, g, st);
+}
+
+namespace {
+// One thread plays both sides of a flag between CTAs.  late 0: gives, then takes.  late 1: takes before anything
+// was given, and gives after that, as a part does whose owner's wait ran out.  out[0]: whether the take saw the
+// flag; out[1]: whether the word is 0 when both are done; out[2]: whether a take of the same token, by a replay
+// whose giver has not come yet, sees a flag.
+__global__ void flag_selftest_kernel(int late, int polls, unsigned long long token, unsigned long long* flag, int32_t* out) {
+  if (!late) flag_give(flag, token);
+  out[0] = flag_take(flag, token, polls);
+  if (late) flag_give(flag, token);
+  out[1] = *flag == 0;
+  out[2] = flag_take(flag, token, polls);
+}
+}  // namespace
+
+KVS_API int kvs_selftest_flag(int32_t late, int32_t polls, uint64_t token, uint64_t* flag, int32_t* out,
+                              kvs_stream_t stream) {
+  if (!flag || !out || late < 0 || late > 1 || polls < 1 || token == 0 || token == ~(uint64_t)0) return KVS_E_ARG;
+  flag_selftest_kernel<<<1, 1, 0, to_cuda(stream)>>>(late, polls, token, reinterpret_cast<unsigned long long*>(flag), out);
+  return launch_rc();
 }

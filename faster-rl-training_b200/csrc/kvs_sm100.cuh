@@ -158,13 +158,31 @@ template <uint32_t R> __device__ __forceinline__ void regs_alloc() {
 }
 
 // ------------------------------------------------------------------ flags between CTAs of one kernel
-__device__ __forceinline__ void st_release_gpu(unsigned long long* p, unsigned long long v) {
-  asm volatile("st.release.gpu.global.u64 [%0], %1;\n" ::"l"(p), "l"(v) : "memory");
-}
 __device__ __forceinline__ unsigned long long ld_acquire_gpu(const unsigned long long* p) {
   unsigned long long v;
   asm volatile("ld.acquire.gpu.global.u64 %0, [%1];\n" : "=l"(v) : "l"(p) : "memory");
   return v;
+}
+__device__ __forceinline__ unsigned long long exchange_gpu(unsigned long long* p, unsigned long long v) {
+  unsigned long long old;
+  asm volatile("atom.exch.acq_rel.gpu.global.b64 %0, [%1], %2;\n" : "=l"(old) : "l"(p), "l"(v) : "memory");
+  return old;
+}
+// Results handed from one thread to another of the same launch through a flag word that holds anything but
+// `token` and ~token before.  One thread gives and one takes, once each; whichever of the two comes second
+// leaves the word 0, also where the taker has given up in between: it then leaves ~token, which tells the giver
+// that nobody will come.  So a launch that is replayed with the same token never finds the flag of an earlier
+// one, even of one whose wait ran out.
+__device__ __forceinline__ void flag_give(unsigned long long* flag, unsigned long long token) {
+  if (exchange_gpu(flag, token) == ~token) *flag = 0;
+}
+// false when the flag is not there after `polls` looks at it
+__device__ __forceinline__ bool flag_take(unsigned long long* flag, unsigned long long token, int polls) {
+  bool there = false;
+  for (int n = 0; n < polls && !there; ++n) there = ld_acquire_gpu(flag) == token;
+  if (!there) there = exchange_gpu(flag, ~token) == token;  // (it came after the last look)
+  if (there) *flag = 0;
+  return there;
 }
 
 // ------------------------------------------------------------------ programmatic dependent launch

@@ -583,6 +583,12 @@ int kvs_selftest_umma(const void* a, const void* b, float* c, int32_t mode, int3
  * (the kernels then record an error and wind down), 0 if it completed; out[1], out[2] = the
  * wait's SM cycles (low, high 32 bits).  A timeout leaves the context usable. */
 int kvs_selftest_wait(int32_t mode, uint32_t limit, int32_t* out, kvs_stream_t stream);
+/* Self-test of the flags by which CTAs of one launch hand partial sums to one another (no reference
+ * counterpart): one thread gives and takes a flag word (late = 0), or takes it, at most `polls` looks, before it
+ * is given (late = 1: a wait that ran out).  out[0] = 1 if the take saw the flag, out[1] = 1 if the word is 0
+ * after both, out[2] = 1 if a second take with the same token sees a flag that nobody gave again. */
+int kvs_selftest_flag(int32_t late, int32_t polls, uint64_t token, uint64_t* flag, int32_t* out,
+                      kvs_stream_t stream);
 
 #ifdef __cplusplus
 }
