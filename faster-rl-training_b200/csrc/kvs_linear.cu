@@ -522,6 +522,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
             there &= flag_take(p.ready + ((pair + r) * 2 + (int)rank) * EPI_WARPS + w, p.token, there ? 1 << 21 : 1);
         }
         if (!__all_sync(0xffffffffu, there)) dead = true;
+        __syncwarp();  // lane 0 acquired the flags; a vote orders no memory, this does, before any lane reads the sums
       }
       const float4* sums = reinterpret_cast<const float4*>(p.sums) +
                            (int64_t)(((pair + 1) * 2 + (int)rank) * EPI_WARPS + w) * (SUMS_PER_WARP / 4) + lane;
