@@ -60,15 +60,23 @@ namespace {
 // (the approximate quotient is good to an ulp or two; 0 past 2^126, where 1 / (1 + e^-z) is below any half step)
 __device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
 
-// The normal distribution function F(z) and e = exp(-z^2 / 2), by Abramowitz and Stegun 7.1.26 (the
-// tail of the error function as e times a polynomial in 1 / (1 + p |z|)): F is off by 7.5e-8 at most.
-// In 32 bits z F(z) is as near as with erff over -9..9 (4.2e-7 against 4.5e-7 at most) and nearer
-// below -4, where 1 + erff(z) cancels; it takes less than half the instructions.
+// The normal distribution function F(z) and e = exp(-z^2 / 2).  For z <= 0, F(z) = e t P(t) with t = 1 / (1 + 0.3 |z|):
+// the tail divided by e is smooth in t (the form of Abramowitz and Stegun 7.1.26).  P is of degree 7, fitted here to the
+// smallest largest relative error over |z| <= 14, 1.5e-7 (iteratively reweighted least squares, Lawson 1961), so the
+// tail is good to a few float32 roundings of itself: z F(z) is within 2e-6 of its value to z = -6 (8e-6 at -13, from the
+// exponent's rounding), where 0.5 z (1 + erff) cancels; for z > 0, 1 - F is that good and F(z) a rounding off.
+// 4096 x 4096 x 1024 with gelu takes 38.8 us, with erff 43.
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
-  const float t = __fdividef(1.f, fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
+  const float t = __fdividef(1.f, fmaf(0.3f, fabsf(z), 1.f));
   e = ex2_approx(-0.72134752044448170f * z * z);
-  float q = fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f);
-  q = __fmul_rn(q, 0.5f * t * e);
+  float q = fmaf(0.03567476044f, t, -0.157203025f);
+  q = fmaf(q, t, 0.2063534069f);
+  q = fmaf(q, t, -0.05368355283f);
+  q = fmaf(q, t, 0.1285615785f);
+  q = fmaf(q, t, 0.09991350659f);
+  q = fmaf(q, t, 0.1207539537f);
+  q = fmaf(q, t, 0.1196292990f);
+  q = __fmul_rn(q, t * e);
   return z > 0.f ? 1.f - q : q;
 }
 
