@@ -57,8 +57,12 @@ using namespace kvs::sm100;
 namespace {
 
 // ------------------------------------------------------------------ element-wise helpers
-// (the approximate quotient is good to an ulp or two; 0 past 2^126, where 1 / (1 + e^-z) is below any half step)
-__device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+// 1 / (1 + e^-z), by t = e^-|z| <= 1 on either side: t becomes subnormal and 0 below z = -87.3, where e^-z passes
+// 2^126 and an approximate quotient by it would be 0 already (silu(-88) = -5.3e-37 is a normal bf16 number)
+__device__ __forceinline__ float sigmoid_f(float z) {
+  const float t = __expf(-fabsf(z));
+  return __fdividef(z < 0.f ? t : 1.f, 1.f + t);  // (good to an ulp or two; a NaN stays one)
+}
 
 // The normal distribution function F(z) and e = exp(-z^2 / 2).  For z <= 0, F(z) = e t P(t) with t = 1 / (1 + 0.3 |z|):
 // the tail divided by e is smooth in t (the form of Abramowitz and Stegun 7.1.26).  P is of degree 7, fitted here to the

@@ -46,3 +46,45 @@ def test_gelu_to_a_rounding(dtype, rows):
     fi = torch.finfo(dtype)
     rel = fi.eps / 2 + 1.5 * zd * zd * 2.0**-24 + 2.0**-19
     assert ((got - want).abs() <= want.abs() * rel + fi.tiny * fi.eps / 2).all()
+
+
+@pytest.mark.parametrize("rows", [8, 600])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_silu_to_a_rounding(dtype, rows):
+    """Down to where silu passes bf16's subnormal numbers, in the plain and the gated form."""
+    from kvstreams import ops
+
+    z = _all_between(-110, 110, dtype)
+    got, zd = _applied(z, "silu", rows).double(), z.double()
+    want = zd * torch.sigmoid(zd)
+    fi = torch.finfo(dtype)
+    rel = fi.eps / 2 + zd.abs() * 2.0**-23 + 2.0**-20
+    bound = want.abs() * rel + fi.tiny * fi.eps / 2 + zd.abs() * 2.0**-149
+    assert ((got - want).abs() <= bound).all()
+    # the same with a factor of 1 (w_up picks a column of ones)
+    eye = torch.eye(64, device="cuda", dtype=dtype)
+    up = torch.zeros_like(eye)
+    up[:, 63] = 1
+    zz = torch.cat([z, z.new_zeros(-z.numel() % (rows * 63))]).view(-1, 63)
+    x = torch.cat([zz, torch.ones_like(zz[:, :1])], 1)
+    h = torch.cat([ops.gated_linear(part, eye, up) for part in x.split(rows)])[:, :63].reshape(-1)[:z.numel()]
+    assert torch.equal(h.double(), got)
+
+
+def test_silu_gradient_below_the_border():
+    """gy silu'(z) = gy s (1 + z (1 - s)) where s is below 2^-126: dx of a product with the identity."""
+    from kvstreams import ops
+
+    z = torch.tensor([-80.0, -86.5, -87.5, -88.0, -88.5, -90.0, 0.0, 88.5], device="cuda").bfloat16()
+    x = z.repeat(8, 8)
+    w = torch.eye(64, device="cuda").bfloat16()
+    pre = ops.pre_buffer(x, 64)
+    ops.linear(x, w, activation="silu", pre=pre)
+    gy = torch.full_like(x, 2.0)
+    dx, _, _ = ops.linear_backward(gy, x, w, pre=pre, activation="silu")
+    zd = x.double().requires_grad_()
+    (want,) = torch.autograd.grad(F.silu(zd), [zd], gy.double())
+    # dz is rounded to bf16, the product with the identity is exact; s good as in silu, 1 + z (1 - s) to 2^-22 of |z|
+    fi = torch.finfo(torch.bfloat16)
+    bound = want.abs() * (fi.eps / 2 + 2.0**-15) + fi.tiny * fi.eps + 200 * 2.0**-149
+    assert ((dx.double() - want).abs() <= bound).all()
