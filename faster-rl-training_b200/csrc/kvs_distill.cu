@@ -254,14 +254,16 @@ distill_kernel(const T* __restrict__ logits, int64_t ld, int n_rows, int vocab, 
     cluster.sync();  // the others' shared memory stays until it is read
     if (seg != 0) return;
   }
-  const A lse = mm * inv_temp + log_full(S);
+  const A logS = log_full(S), lse = mm * inv_temp + logS;
   const A logz = log_full(sum[1]);
   A term[1] = {A(0)};
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     if (slot.id[u] < 0) continue;
+    // log q by the distance to the row's largest: the loss does not change with a shift of the row, and
+    // x / T - lse would carry half a step of lse (5e-4 at logits near 1e4)
     const A lp = e[u] - logz, p = exp_full(lp);
-    if (p != A(0)) term[0] += p * (lp - (to_acc<T>(xs[u]) * inv_temp - lse));
+    if (p != A(0)) term[0] += p * (lp - ((to_acc<T>(xs[u]) - mm) * inv_temp - logS));
   }
   group_reduce<G, SumOp>(term, red);
   if (tid == 0) {

@@ -563,7 +563,8 @@ int kvs_distill(const void* logits, int64_t ld, int32_t n_rows, int32_t vocab, c
 /* Its gradient with respect to the logits for upstream grad[r] (type of lse) with the forward's lse:
  * dlogits[r][v] = grad[r] (exp(x[r][v]/T - lse[r]) - sum_{j: id_j = v} p_j) / T, zeros for a row
  * without kept slots; in out_dtype (the logits' own, or KVS_BF16 / KVS_F16 from KVS_F32) with row
- * stride ld_out.  dlogits may be the logits buffer itself when dtype and stride are its own. */
+ * stride ld_out.  dlogits may be the logits buffer itself when dtype and stride are its own.  (lse comes rounded to
+ * its type: the softmax is good to half a step of lse, 2^-24 |lse| relative in float; the loss does not use it.) */
 int kvs_distill_backward(const void* logits, int64_t ld, int32_t n_rows, int32_t vocab, const int64_t* ids,
                          const void* teacher, int32_t top, const void* lse, const void* grad, double temperature,
                          int32_t dtype, void* dlogits, int64_t ld_out, int32_t out_dtype, kvs_stream_t stream);
