@@ -4,7 +4,9 @@
 74-86 of the reference) with bias, activation, gate product and residual in the product's own
 launch; :func:`distill` is the loss of logits rows against a teacher's top logits.  Each is one
 autograd node over the pair of kernels in :mod:`kvstreams.ops`; only the gradients that are
-needed are computed, and what an activation's gradient needs is kept in float32.
+needed are computed, and what an activation's gradient needs is kept in float32, where autograd
+records: a node's ``needs_input_grad`` is true for a parameter under ``torch.no_grad()`` too, so the
+mode is asked before the node (whose forward always runs with recording off).
 
 Capturing a backward pass into a CUDA graph: PyTorch ties the accumulation into a leaf to the stream
 of the leaf's first use, so release every eager graph over the same leaves before the capture (or
@@ -32,9 +34,9 @@ def product_kernels(x: torch.Tensor, *weights: torch.Tensor) -> bool:
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation):
+    def forward(ctx, x, weight, bias, residual, activation, recorded):
         pre = None
-        if activation is not None and any(ctx.needs_input_grad[:3]):
+        if recorded and activation is not None and any(ctx.needs_input_grad[:3]):
             pre = ops.pre_buffer(x, weight.shape[0])
         y = ops.linear(x, weight, bias=bias, residual=residual, activation=activation, pre=pre)
         ctx.save_for_backward(x, weight, pre)
@@ -45,18 +47,18 @@ class _Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gy):
         x, weight, pre = ctx.saved_tensors
-        nx, nw, nb, nr, _ = ctx.needs_input_grad
+        nx, nw, nb, nr = ctx.needs_input_grad[:4]
         dx = dw = db = None
         if nx or nw or nb:
             dx, dw, db = ops.linear_backward(gy, x, weight, pre=pre, activation=ctx.activation, bias_grad=nb,
                                              need_dx=nx, need_dw=nw)
-        return dx, dw, db, gy if nr else None, None
+        return dx, dw, db, gy if nr else None, None, None
 
 
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, activation):
-        pre = ops.pre_buffer(x, 2 * w_gate.shape[0]) if any(ctx.needs_input_grad[:3]) else None
+    def forward(ctx, x, w_gate, w_up, activation, recorded):
+        pre = ops.pre_buffer(x, 2 * w_gate.shape[0]) if recorded and any(ctx.needs_input_grad[:3]) else None
         h = ops.gated_linear(x, w_gate, w_up, activation=activation, pre=pre)
         ctx.save_for_backward(x, w_gate, w_up, pre)
         ctx.activation = activation
@@ -66,10 +68,10 @@ class _GatedLinear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gh):
         x, w_gate, w_up, pre = ctx.saved_tensors
-        nx, ng, nu, _ = ctx.needs_input_grad
+        nx, ng, nu = ctx.needs_input_grad[:3]
         dx, dg, du = ops.gated_linear_backward(gh, x, w_gate, w_up, pre, activation=ctx.activation, need_dx=nx,
                                                need_dw=ng or nu)
-        return dx, dg if ng else None, du if nu else None, None
+        return dx, dg if ng else None, du if nu else None, None, None
 
 
 class _Distill(torch.autograd.Function):
@@ -91,14 +93,14 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
            residual: Optional[torch.Tensor] = None, activation: Optional[str] = None) -> torch.Tensor:
     """``act(x @ weight.T + bias) + residual`` (:func:`kvstreams.ops.linear`), differentiable in x,
     weight, bias and residual."""
-    return _Linear.apply(x, weight, bias, residual, activation)
+    return _Linear.apply(x, weight, bias, residual, activation, torch.is_grad_enabled())
 
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
                  activation: Optional[str] = "silu") -> torch.Tensor:
     """``act(x @ w_gate.T) * (x @ w_up.T)`` (:func:`kvstreams.ops.gated_linear`), differentiable in x
     and both weights."""
-    return _GatedLinear.apply(x, w_gate, w_up, activation)
+    return _GatedLinear.apply(x, w_gate, w_up, activation, torch.is_grad_enabled())
 
 
 def distill(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
