@@ -1232,11 +1232,14 @@ template <typename K> int max_pairs(K kernel, KernelState& s) {
 //
 // Pairs with cut units are at different K blocks and share operands only through L2, of which about
 // 90 MB holds them (110 where both operands lie MN-major: a K block of all tiles is then contiguous):
-// what does not fit comes from HBM again for every pair, 64 KB a K block.  Units are cut where the
-// larger of the two times gains four percent.  Weight gradients, whole tiles against cut: 4096 x 4096
+// what does not fit comes from HBM again for every pair, 64 KB a K block of a full tile.  Units are cut where
+// the larger of the two times gains four percent.  Weight gradients, whole tiles against cut: 4096 x 4096
 // from 8192 rows 239 -> 220 us, from 16384 532 -> 439, 6144 x 4096 from 16384 782 -> 674; forward
 // 4000 x 2560 x 8192 172 -> 138.  Not cut: a 4096 x 4096 weight gradient from 32768 rows (971 us,
-// cut 1065), 2048 x 4096 x 14336 (165, cut 231), 8192 x 4096 over 28672 (1885, cut 2050).
+// cut 1065), 2048 x 4096 x 14336 (165, cut 231), 8192 x 4096 over 28672 (1885, cut 2050): past 250 MB only in
+// equal cuts, at most half as many units as pairs, whose pairs stay as near in K as those of whole units do and
+// which would leave the others idle (weight gradients of a narrow layer, whole tiles against cut: 64 x 64 from
+// 262144 rows 1097 -> 99 us, 1 x 4096 from 65536 291 -> 120, 1001 x 520 from 131072 567 -> 190).
 constexpr int PAIRS = 74;  // of a B200's 148 SMs
 struct PairPlan {
   int bn, whole, cut_pairs;
@@ -1251,7 +1254,8 @@ int group_of(int64_t N, int kb, bool gated) {
   const int64_t row = 2 * (int64_t)kb * BK;  // bytes
   return N * (gated ? 2 : 1) * row > (48 << 20) && 16 * 256 * row <= (48 << 20) ? 16 : 8;
 }
-PairPlan pair_plan(int64_t row_blocks, int64_t N, int kb, bool gated, bool both_mn, bool cut_allowed) {
+PairPlan pair_plan_of(int64_t M_part, int m_parts, int64_t N, int kb, bool gated, bool both_mn, bool cut_allowed) {
+  const int64_t M = M_part * m_parts, row_blocks = (M_part + 2 * BM - 1) / (2 * BM) * m_parts;
   auto units_of = [&](int bn) { return row_blocks * ((N + (gated ? bn / 2 : bn) - 1) / (gated ? bn / 2 : bn)); };
   auto rounds = [](int64_t units) { return (double)((units + PAIRS - 1) / PAIRS); };
   const int64_t units = units_of(256);
@@ -1260,12 +1264,14 @@ PairPlan pair_plan(int64_t row_blocks, int64_t N, int kb, bool gated, bool both_
   if (narrow < best.us) best = {128, (int)std::min<int64_t>(units_of(128), 1 << 30), 0, narrow};
   if (!cut_allowed || units % PAIRS == 0 || units >= (1 << 30)) return best;
   const int64_t whole = std::max<int64_t>(0, units / PAIRS - 1) * PAIRS, rest = units - whole;
-  const int64_t cols = units / row_blocks;
+  // bytes that the cut units' tiles read, in rows and columns that exist, and a K block of one of them
+  const int64_t cols = units / row_blocks, n_cols = gated ? 2 * N : N;
   const int64_t r = std::max(std::min<int64_t>(row_blocks, group_of(N, kb, gated)), (rest + cols - 1) / cols);
   const int64_t c = std::min(cols, (rest + r - 1) / r);
-  const double shared_mb = (double)(r + c) * 256 * kb * BK * 2 / 1e6, fits_mb = both_mn ? 110.0 : 90.0;
-  if (shared_mb > 250.0) return best;
-  const double hbm_us = shared_mb > fits_mb ? (double)rest * kb * 65536.0 * (1.0 - fits_mb / shared_mb) / 6.4e6 : 0.0;
+  const double shared_mb = (double)(std::min(r * 256, M) + std::min(c * 256, n_cols)) * kb * BK * 2 / 1e6;
+  const double block_mb = (double)(std::min<int64_t>(256, M) + std::min<int64_t>(256, n_cols)) * BK * 2 / 1e6;
+  const double fits_mb = both_mn ? 110.0 : 90.0;
+  const double hbm_us = shared_mb > fits_mb ? (double)rest * kb * block_mb * (1.0 - fits_mb / shared_mb) / 6.4 : 0.0;
   const double uncut = best.us;
   auto consider = [&](int64_t pairs, int others, bool in_step) {
     const double run = (double)rest * kb / pairs;  // K blocks a pair
@@ -1274,14 +1280,11 @@ PairPlan pair_plan(int64_t row_blocks, int64_t N, int kb, bool gated, bool both_
                       1.5 * (1 + (run > kb)) + 7.0 * (double)pairs / PAIRS + 2.0 * others;
     if (us < best.us && us < 0.96 * uncut) best = {256, (int)whole, (int)pairs, us};
   };
-  // equal cuts of every unit (pairs with the same part of theirs keep in step), or all pairs whatever
-  // the cuts come to
+  // equal cuts of every unit (pairs with the same part of theirs keep in step, whatever the length), or all pairs
+  // whatever the cuts come to
   for (int s = 2; rest < PAIRS && rest * s <= PAIRS; ++s) consider(rest * s, s - 1, true);
-  consider(PAIRS, rest >= PAIRS ? 1 : (int)((PAIRS + rest - 1) / rest), false);
+  if (shared_mb <= 250.0) consider(PAIRS, rest >= PAIRS ? 1 : (int)((PAIRS + rest - 1) / rest), false);
   return best;
-}
-PairPlan pair_plan_of(int64_t M, int m_parts, int64_t N, int kb, bool gated, bool both_mn, bool cut_allowed) {
-  return pair_plan((M + 2 * BM - 1) / (2 * BM) * m_parts, N, kb, gated, both_mn, cut_allowed);
 }
 
 struct Product {
