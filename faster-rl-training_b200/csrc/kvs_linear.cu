@@ -233,6 +233,11 @@ __device__ __forceinline__ bool part_of(const PairParams& p, int kb_all, int pai
   return s.k0 < s.k1;
 }
 
+// Polls, of about 4 us, that a wait for the sums of a run of K blocks may take: the default bound, and 1 us for each
+// block, which takes 0.3 (2^24 blocks, the most that a product has, take longer than the default bound where one pair
+// has them all: a product without scratch, or on fewer SMs than a whole B200's)
+__device__ __forceinline__ uint32_t run_polls(int blocks) { return 400000u + (uint32_t)blocks / 4; }
+
 // unit -> (result, row block, column block): `group` row blocks x all columns at a time, so that
 // the units in flight read few rows of A and few rows of B
 __device__ __forceinline__ void unit_of(const PairParams& p, int u, int& part, int& mb, int& nb) {
@@ -488,7 +493,8 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
       };
       const bool owner = seg.k0 == 0;
       if (res && owner) load_res(0);
-      if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(&bar[B_ACCF + ab], (ui >> 1) & 1, abort_flag));
+      if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(&bar[B_ACCF + ab], (ui >> 1) & 1, abort_flag,
+                                                                      run_polls(seg.k1 - seg.k0)));
       if (dead && lane == 0) *abort_flag = 1;
       tc_fence_after();
       const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + ab * BN + half * COLS;
@@ -855,7 +861,7 @@ stream_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_const
     // partial sums to shared memory, [row of x][128 weight rows]: over the ring,
     // which nothing uses any more once the last MMA has completed
     const int q = warp & 3;  // TMEM lane quadrant
-    const bool ok = __all_sync(0xffffffffu, mbar_wait(done, 0, abort_flag));
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(done, 0, abort_flag, run_polls(kb_end - kb_beg)));
     if (!ok) {  // the NaNs go where copies may still be landing: after those
       if (lane == 0) *abort_flag = 1;
       mbar_wait(drained, 0, nullptr);
