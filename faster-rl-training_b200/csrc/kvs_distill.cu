@@ -143,7 +143,7 @@ __device__ __forceinline__ void pack_sum(const Pack<double>& q, double c, double
 // s = sum of exp((x - m) / T).  16-byte loads between the ends, kUnroll of them in flight, one
 // rescale of the sum per batch.
 template <int G, typename T, typename A>
-__device__ void row_lse(const T* __restrict__ x, int n, A c, int tid, A& m, A& s) {
+__device__ void row_lse(const T* x, int n, A c, int tid, A& m, A& s) {
   using P = Pack<T>;
   constexpr int kUnroll = 4;
   auto raise = [&](A xm) {  // the reference for a batch whose largest element is xm
@@ -164,7 +164,7 @@ __device__ void row_lse(const T* __restrict__ x, int n, A c, int tid, A& m, A& s
     P q[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-      if (i0 + u * G < packs) *reinterpret_cast<uint4*>(&q[u]) = __ldg(reinterpret_cast<const uint4*>(xp + i0 + u * G));
+      if (i0 + u * G < packs) *reinterpret_cast<uint4*>(&q[u]) = *reinterpret_cast<const uint4*>(xp + i0 + u * G);
     A bm = pack_max(q[0]);
 #pragma unroll
     for (int u = 1; u < kUnroll; ++u)
@@ -184,12 +184,14 @@ __device__ void row_lse(const T* __restrict__ x, int n, A c, int tid, A& m, A& s
   if (tail < n) one(x[tail]);  // fewer than P::n <= G elements
 }
 
+// (No __restrict__ on what these kernels read: a kernel that starts before the one before it has ended may not load
+// that one's results as read-only data, nor may the compiler move the loads up past the wait as such.)
+//
 // Grid: rows / (256 / G) CTAs of one row group each, times `segs` CTAs (one cluster) per row.
 template <typename T, typename A, int G, int PER>
 __global__ void __launch_bounds__(kThreads)
-distill_kernel(const T* __restrict__ logits, int64_t ld, int n_rows, int vocab, const int64_t* __restrict__ ids,
-               const A* __restrict__ teacher, int top, A inv_temp, A c, int segs, A* __restrict__ loss,
-               A* __restrict__ lse_out) {
+distill_kernel(const T* logits, int64_t ld, int n_rows, int vocab, const int64_t* ids, const A* teacher, int top,
+               A inv_temp, A c, int segs, A* loss, A* lse_out) {
   __shared__ A red[3 * (kThreads / 32)];
   __shared__ A part[2];
   sm100::pdl_let_next_start();
@@ -295,9 +297,8 @@ template <typename O, typename A, int N> __device__ __forceinline__ void put(O* 
 // needs of it (the entries that slots name).
 template <typename T, typename A, typename O, int G, int PER>
 __global__ void __launch_bounds__(kThreads)
-distill_bwd_kernel(const T* logits, int64_t ld, int n_rows, int vocab, const int64_t* __restrict__ ids,
-                   const A* __restrict__ teacher, int top, const A* __restrict__ lse_in, const A* __restrict__ grad,
-                   A inv_temp, A c, int segs, O* dlogits, int64_t ld_out) {
+distill_bwd_kernel(const T* logits, int64_t ld, int n_rows, int vocab, const int64_t* ids, const A* teacher, int top,
+                   const A* lse_in, const A* grad, A inv_temp, A c, int segs, O* dlogits, int64_t ld_out) {
   constexpr int TOP = G * PER;  // slots of a row at most
   __shared__ A red[2 * (kThreads / 32)];
   __shared__ A sp_all[kThreads / G][TOP];

@@ -989,6 +989,8 @@ stream_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_const
 }
 
 // ------------------------------------------------------------------ gradients of the epilogue
+// (No __restrict__ on what these kernels read: a kernel that starts before the one before it has ended may not load
+// that one's results as read-only data, nor may the compiler move the loads up past the wait as such.)
 // Eight consecutive elements as they lie in memory: as separate half-precision values they would
 // be unpacked, and waited for, where they are loaded.
 template <typename T> struct alignas(16) Raw8 {
@@ -1019,8 +1021,8 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float (
 // gradient 47 us (268 MB, 5.7 TB/s).
 template <typename T, typename Z>
 __global__ void __launch_bounds__(256, 4)
-dz_kernel(const T* __restrict__ gy, int64_t ld_gy, const Z* __restrict__ pre, int64_t ld_pre, int act,
-          T* __restrict__ dz, int64_t ld_dz, float* __restrict__ part, int M, int N, int rows_per, int vec) {
+dz_kernel(const T* gy, int64_t ld_gy, const Z* pre, int64_t ld_pre, int act, T* dz, int64_t ld_dz, float* part, int M,
+          int N, int rows_per, int vec) {
   __shared__ float red[4][512];
   pdl_let_next_start();
   pdl_wait_for_previous();
@@ -1080,7 +1082,7 @@ dz_kernel(const T* __restrict__ gy, int64_t ld_gy, const Z* __restrict__ pre, in
 // added in order
 template <typename T>
 __global__ void __launch_bounds__(256)
-bias_grad_kernel(const float* __restrict__ part, T* __restrict__ db, int n_parts, int N) {
+bias_grad_kernel(const float* part, T* db, int n_parts, int N) {
   __shared__ float red[8][32];
   pdl_let_next_start();
   pdl_wait_for_previous();
@@ -1104,8 +1106,8 @@ bias_grad_kernel(const float* __restrict__ part, T* __restrict__ db, int n_parts
 // at `half` (N rounded up to 8), zeros between.  Bound by HBM.
 template <typename T, typename Z>
 __global__ void __launch_bounds__(256)
-gated_dz_kernel(const T* __restrict__ gh, int64_t ld_gh, const Z* __restrict__ pre, int64_t ld_pre, int act,
-                T* __restrict__ dgu, int64_t ld_dgu, int half, int64_t M, int N, int vec) {
+gated_dz_kernel(const T* gh, int64_t ld_gh, const Z* pre, int64_t ld_pre, int act, T* dgu, int64_t ld_dgu, int half,
+                int64_t M, int N, int vec) {
   pdl_let_next_start();
   pdl_wait_for_previous();
   const int nvec = half / 8;
