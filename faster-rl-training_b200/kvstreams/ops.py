@@ -768,6 +768,8 @@ def distill_backward(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Ten
     elif (tuple(out.shape) != (n, vocab) or out.device != logits.device or out.dtype != (out_dtype or out.dtype)
           or (vocab > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < vocab)):
         raise ValueError(f"out must be [{n}, {vocab}] with dense rows on {logits.device}, of type {out_dtype}")
+    elif any(_overlap(out, v) for v in (i, t, l, g)):
+        raise ValueError("out overlaps ids, teacher, lse or grad")
     if out.dtype not in N.DTYPE_CODE:
         raise ValueError(f"unsupported gradient dtype {out.dtype}")
     _launch(logits, N.launch_lib().kvs_distill_backward, "kvs_distill_backward", logits.data_ptr(), ld, n, vocab,
