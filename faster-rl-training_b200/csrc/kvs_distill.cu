@@ -362,7 +362,9 @@ distill_bwd_kernel(const T* logits, int64_t ld, int n_rows, int vocab, const int
     for (int i = head + packs * P::n + tid; i < len; i += G) d[beg + i] = round_to<O, A>(one);
     return;
   }
-  // the first slot of an id takes the sum of all its slots, in slot order
+  // the first slot of an id takes the sum of all its slots, in slot order.  (Every slot is compared with every
+  // other, top^2 / G steps a thread: hidden at 128 slots, not past 256: 4096 x 128256 float32 to a bf16 gradient
+  // takes 496 us with 64 slots, 509 with 128, 539 with 256, 760 with 512, 1780 with 1024.)
   const A gz = g / sum[0];
   A val[PER];
   int at[PER];
@@ -417,7 +419,7 @@ constexpr int kWarpRowBytes = 4096;
 template <typename T> bool warp_rows(int vocab, int top) {
   return (int64_t)vocab * (int64_t)sizeof(T) <= kWarpRowBytes && top <= kWarpTop;
 }
-// CTAs per row: doubled while the rows give the machine less than eight CTAs an SM and a segment
+// CTAs per row: doubled while the rows give the machine less than four CTAs an SM and a segment
 // keeps 8 KB (two 16-byte loads a thread)
 template <typename T> int segments(int vocab, int n_rows) {
   int s = 1;

@@ -704,8 +704,9 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constan
 // places: 128 weight rows (or, in dx, 128 columns of W) are the M = 128 rows of the MMA and a tile
 // of 16..128 rows of x its N columns, so the tensor cores' work follows the rows that exist and
 // TMEM lane = result column.  A cluster of S CTAs takes one tile and splits the reduced index
-// between them, so that (result tiles x S) CTAs stream the weights at once, one per SM or two, each with
-// about 200 or 100 KB of copies in flight (stream_plan has the rule and both sides' times).  The S
+// between them, so that (result tiles x S) CTAs stream the weights at once, one per SM (147 KB of copies in
+// flight at 16 rows, eight stages, to 229 KB at 128) or two (98 to 111 KB each); stream_plan has the rule and both
+// sides' times.  The S
 // partial sums meet in distributed shared memory: CTA r adds up, in rank order, the 128 / S result
 // columns that it then finishes (bias, activation, gate product, residual) and stores.  Nothing
 // passes through global memory, no counters, no second launch, and the order of the sum is fixed.
@@ -1232,11 +1233,19 @@ template <typename K> int max_pairs(K kernel, KernelState& s) {
 }
 
 // How a product is dealt out to the CTA pairs: unit width, units done whole, pairs that share the
-// K blocks of the others, and the estimate in microseconds by which the cut was chosen (B200,
-// measured at 512..8192 x 4096 x 4096).  About 6 outside the loop, 1.5 a unit, and per K block
-// 0.29 for 256 columns, which the tensor cores bound, but 0.235 for 128, which the 64 bytes per clock
+// K blocks of the others, and the estimate in microseconds by which the cut was chosen: of a single
+// launch at full clock whose operands come from L2.  About 6 outside the loop, 1.5 a unit, and per K block
+// 0.29 for 256 columns, near the tensor cores' nominal rate, but 0.235 for 128, which the 64 bytes per clock
 // that an SM takes from L2 bound (24 KB a block against 32).  Cut units cost about 7 (19 MB of sums
 // written at once; less with fewer pairs) and 2 for each pair whose sums the last one to finish has to add.
+//
+// The estimates compare ways of one product; they are not its time.  Fitted on 512..2048 x 4096 x 4096, they come
+// out low as products grow, since the clock falls under the power cap and long reduced indexes wait for HBM:
+// 8192 x 4096 x 4096 146 (measured 168-199), 4096 x 14336 gated x 4096 507 (590), 1999 x 6144 x 4096 66 (69-90),
+// a 4096 x 4096 weight gradient from 16384 rows whole 309 (532), from 32768 606 (790-970).  What they chose, whole
+// tiles against cut: 1024 x 6144 x 4096 46 -> 43 us, 2048 x 2560 x 4096 46 -> 37, 640 x 4096 x 14336 99 -> 81,
+// 2304 x 2304 x 16384 168 -> 159, 900 x 1500 x 14344 76 -> 50, 300 x 2048 x 32768 139 -> 63; of 12 sizes cut one
+// lost, 3000 x 2560 x 8192 91 -> 96.
 //
 // Pairs with cut units are at different K blocks and share operands only through L2, of which about
 // 90 MB holds them (110 where both operands lie MN-major: a K block of all tiles is then contiguous):
