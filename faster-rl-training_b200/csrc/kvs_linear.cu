@@ -1318,7 +1318,7 @@ unsigned long long launch_token() {
   z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
   z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
   z ^= z >> 31;
-  return z && ~z ? z : 1;  // (0 is the word of a flag that is not set, ~0 that of one given up)
+  return z && ~z ? z : 1;  // (a clean word, 0, is neither a token nor the complement that a given-up flag holds)
 }
 
 template <typename T, bool A_MN, bool B_MN, int EPI, int BN>

@@ -268,7 +268,8 @@ class TinyLM(nn.Module):
         (:mod:`kvstreams.functional`): q|k|v, output projection + residual, gate/up/silu/product in
         one launch, down projection + residual, and their gradients.  Off by default: the layers
         then use PyTorch's products, whose results differ by the rounding of gate|up and of the
-        gradients' operands.  Layers of other types or sizes keep PyTorch's products either way."""
+        gradients' operands.  Layers of other types or sizes keep PyTorch's products either way; CUDA
+        graphs keep the products that they were recorded with."""
         return bool(self.__dict__.get("_fused_products", False))
 
     @fused_products.setter

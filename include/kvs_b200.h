@@ -496,8 +496,8 @@ int kvs_silu_mul_backward(const void* gu, const void* grad, void* dgu, int64_t n
  * [rows][n], or [rows][2 n] = gate | up, in pre_dtype (KVS_F32, or dtype: half the memory, one more
  * rounding in the gradients).  out may be the residual.
  * Any rows (0: nothing happens; at most 2^30) and n (at most 2^29); k (at most 2^30) and the pitches of
- * x and the weights multiples of 8, their bases 16-byte aligned (KVS_E_UNSUPPORTED otherwise).  A bounded wait inside a kernel that runs
- * out gives NaN outputs. */
+ * x and the weights multiples of 8, their bases 16-byte aligned (KVS_E_UNSUPPORTED otherwise).  A bounded
+ * wait inside a kernel that runs out gives NaN outputs. */
 enum kvs_activation { KVS_ACT_NONE = 0, KVS_ACT_RELU = 1, KVS_ACT_SILU = 2, KVS_ACT_GELU = 3 /* erf form */ };
 typedef struct kvs_linear_args {
   const void* x;
@@ -532,7 +532,8 @@ int kvs_linear(const kvs_linear_args* a, kvs_stream_t stream);
  * db [n], each written when its pointer is given (rows of dw and dw_up are ld_dw apart; gated needs
  * dw and dw_up together and has no db).  a: x and the weights as in the forward, pre as the forward
  * wrote it (needed when gated or with an activation); bias, residual and out are not read.  The
- * gradient of the residual is gy itself.  Sums run in a fixed order (no float atomics).
+ * gradient of the residual is gy itself.  Outputs and scratch may not overlap what is read, nor one another.
+ * Sums run in a fixed order (no float atomics).
  * scratch: kvs_linear_backward_scratch_bytes(a, g) bytes, 256-byte aligned. */
 typedef struct kvs_linear_grads {
   const void* gy;
