@@ -69,7 +69,8 @@ __device__ __forceinline__ float sigmoid_f(float z) {
 // smallest largest relative error over |z| <= 14, 1.5e-7 (iteratively reweighted least squares, Lawson 1961), so the
 // tail is good to a few float32 roundings of itself: z F(z) is within 2e-6 of its value to z = -6 (8e-6 at -13, from the
 // exponent's rounding), where 0.5 z (1 + erff) cancels; for z > 0, 1 - F is that good and F(z) a rounding off.
-// 4096 x 4096 x 1024 with gelu takes 38.8 us, with erff 43.
+// 4096 x 4096 x 1024 with gelu takes 38.8 us, with erff 43; gated 4096 x 14336 x 4096 611, with 7.1.26 itself, which is
+// three multiply-adds shorter and 0.3 % off in the tail, 606.
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
   const float t = __fdividef(1.f, fmaf(0.3f, fabsf(z), 1.f));
   e = ex2_approx(-0.72134752044448170f * z * z);
